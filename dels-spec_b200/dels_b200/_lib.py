@@ -24,6 +24,10 @@ DELS_ERR_DEVICE_TIMEOUT = -6
 DELS_ACT_IDENTITY = 0
 DELS_ACT_SILU = 1
 DELS_FLAG_KEYS_READY = 1
+DELS_DTYPE_BF16 = 0
+DELS_DTYPE_F32 = 1
+DELS_BEAM_MAX = 64
+DELS_BEAM_MAX_VOCAB = 524288
 DELS_WS_HEADER_BYTES = 256
 DELS_NOALLOC_SCRATCH_BYTES = 12 * 1024 * 1024
 
@@ -92,6 +96,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dels_linear_bf16": (_I, [_P, _I64, _P, _I64, _P, _I, _I, _I, _P, _I64, _P, _SZ, _P]),
     "dels_correction_mid_bf16": (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P, _P, _P]),
     "dels_correction_mid_tc_bf16": (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P, _P, _SZ, _P]),
+    "dels_beam_select_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "dels_beam_select": (
+        _I,
+        [_P, _I, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _SZ, _P],
+    ),
+    "dels_beam_reorder": (_I, [_P, _I, _P, _I, _I, _I, _P, _P]),
     "dels_selftest_bounded_wait": (_I, [_P, _P, ctypes.c_double, _P]),
     "dels_draft_score_bf16_noalloc": (
         _I,

@@ -11,6 +11,7 @@
 #include <utility>
 #include <string>
 
+#include "beam_kernels.cuh"
 #include "f32_score.cuh"
 #include "runner_kernels.cuh"
 #include "small_kernels.cuh"
@@ -196,6 +197,8 @@ cudaError_t set_smem(K kernel, int bytes) {
 }
 
 constexpr int kMaxSmem = 232448;
+constexpr int kBeamRowSmemMax = kBeamMax * kBeamGroup * (int)sizeof(uint32_t);
+static_assert(kBeamMaxGroups * (int)sizeof(uint32_t) <= kBeamRowSmemMax, "group keys fit");
 
 int init_device(int dev) {
   if (dev < 0 || dev >= kMaxDevices) return fail(DELS_ERR_INVALID_ARG, "device %d out of range", dev);
@@ -259,6 +262,20 @@ int init_device(int dev) {
     SET(gru_gates_kernel, 0);
     SET(gru_finalize_kernel, 0);
     SET(wait_selftest_kernel, 0);
+    SET((beam_scan_kernel<float, false, false>), 0);
+    SET((beam_scan_kernel<float, false, true>), 0);
+    SET((beam_scan_kernel<float, true, false>), 0);
+    SET((beam_scan_kernel<float, true, true>), 0);
+    SET((beam_scan_kernel<__nv_bfloat16, false, false>), 0);
+    SET((beam_scan_kernel<__nv_bfloat16, false, true>), 0);
+    SET((beam_scan_kernel<__nv_bfloat16, true, false>), 0);
+    SET((beam_scan_kernel<__nv_bfloat16, true, true>), 0);
+    SET((beam_row_kernel<float, false>), kBeamRowSmemMax);
+    SET((beam_row_kernel<float, true>), kBeamRowSmemMax);
+    SET((beam_row_kernel<__nv_bfloat16, false>), kBeamRowSmemMax);
+    SET((beam_row_kernel<__nv_bfloat16, true>), kBeamRowSmemMax);
+    SET(beam_merge_kernel, kBeamMax * kBeamMax * (int)sizeof(uint32_t));
+    SET(beam_reorder_kernel, 0);
 #undef SET
   }
   if (rc == DELS_OK) {
@@ -670,6 +687,76 @@ int fused_argmax_common(const void* h, long long ld_h, const void* W, long long 
   }
   if (vec_base) return launch_tc<256, kArgmax, true>(op, a, ds->sm_count, st);
   return launch_tc<256, kArgmax, false>(op, a, ds->sm_count, st);
+}
+
+// Lays out the scratch of a selection over `base` (counted only when `a` is null); returns
+// its bytes.
+size_t beam_scratch(int n_seq, int beams, int select, int V, char* base, BeamSelectArgs* a) {
+  const size_t rows = (size_t)n_seq * beams;
+  const int groups = cdiv(V, kBeamGroup);
+  // enough CTAs to fill the device several times over, and at least one group for each warp
+  const int per_cta = kBeamThreads / 32;
+  const long long want = rows < 8ll * kTargetCtas ? cdiv(8ll * kTargetCtas, (long long)rows) : 1;
+  const int most = cdiv(groups, per_cta);
+  const int slices = want < most ? (int)want : most;
+  size_t at = 0;
+  const size_t key0 = at;
+  at += align256(rows * groups * sizeof(uint32_t));
+  const size_t part0 = at;
+  at += align256(rows * slices * sizeof(float2));
+  const size_t best0 = at;
+  at += align256(rows * select * sizeof(BeamEntry));
+  const size_t stat0 = at;
+  at += align256(rows * sizeof(float2));
+  if (a != nullptr) {
+    a->groups = groups;
+    a->slices = slices;
+    a->ws.group_key = reinterpret_cast<uint32_t*>(base + key0);
+    a->ws.part = reinterpret_cast<float2*>(base + part0);
+    a->ws.best = reinterpret_cast<BeamEntry*>(base + best0);
+    a->ws.stat = reinterpret_cast<float2*>(base + stat0);
+  }
+  return at;
+}
+
+template <typename T, bool MIX>
+int launch_beam_select(const BeamSelectArgs& a, bool vec, cudaStream_t st) {
+  const int rows = a.n_seq * a.beams;
+  DELS_CHECK_PDL("beam_scan_kernel launch",
+                 launch_pdl(vec ? beam_scan_kernel<T, MIX, true> : beam_scan_kernel<T, MIX, false>,
+                            dim3((unsigned)(rows * a.slices)), dim3(kBeamThreads), 0, st, a));
+  const int group_keys = a.select * kBeamGroup > a.groups ? a.select * kBeamGroup : a.groups;
+  DELS_CHECK_PDL("beam_row_kernel launch", launch_pdl(beam_row_kernel<T, MIX>, dim3((unsigned)rows),
+                                                      dim3(kBeamThreads), group_keys * sizeof(uint32_t), st, a));
+  DELS_CHECK_PDL("beam_merge_kernel launch",
+                 launch_pdl(beam_merge_kernel, dim3((unsigned)a.n_seq), dim3(kBeamThreads),
+                            (size_t)a.beams * a.select * sizeof(uint32_t), st, a));
+  return DELS_OK;
+}
+
+int check_beam_state(const dels_beam_state& d, int i, int n_seq, int beams, int select) {
+  if (d.outer < 0 || d.outer > INT32_MAX || d.inner_bytes < 0)
+    return fail(DELS_ERR_INVALID_ARG, "state %d: bad shape outer=%lld inner=%lld", i, (long long)d.outer,
+                (long long)d.inner_bytes);
+  if (n_seq == 0 || d.outer == 0 || d.inner_bytes == 0) return DELS_OK;
+  if (d.src == nullptr || d.dst == nullptr) return fail(DELS_ERR_INVALID_ARG, "state %d: NULL pointer", i);
+  const long long src_outer = d.outer > 1 ? d.src_outer_stride : 0, dst_outer = d.outer > 1 ? d.dst_outer_stride : 0;
+  const long long src_rows = (long long)n_seq * beams, dst_rows = (long long)n_seq * select;
+  if (d.src_row_stride < 0 || d.dst_row_stride < 0 || src_outer < 0 || dst_outer < 0)
+    return fail(DELS_ERR_INVALID_ARG, "state %d: negative stride", i);
+  // every run of dst is written by its own thread block, so no two may share a byte
+  const long long run = d.inner_bytes;
+  const bool rows_outside = (d.outer == 1 || dst_outer >= run) &&
+                            (dst_rows == 1 || d.dst_row_stride >= (d.outer - 1) * dst_outer + run);
+  const bool rows_inside = (dst_rows == 1 || d.dst_row_stride >= run) &&
+                           (d.outer == 1 || dst_outer >= (dst_rows - 1) * d.dst_row_stride + run);
+  if (!rows_outside && !rows_inside) return fail(DELS_ERR_INVALID_ARG, "state %d: rows of dst overlap", i);
+  const uintptr_t s0 = reinterpret_cast<uintptr_t>(d.src), d0 = reinterpret_cast<uintptr_t>(d.dst);
+  if (s0 == d0 && beams == select && d.src_row_stride == d.dst_row_stride && src_outer == dst_outer) return DELS_OK;
+  const uintptr_t s1 = s0 + (src_rows - 1) * d.src_row_stride + (d.outer - 1) * src_outer + run;
+  const uintptr_t d1 = d0 + (dst_rows - 1) * d.dst_row_stride + (d.outer - 1) * dst_outer + run;
+  if (s0 < d1 && d0 < s1) return fail(DELS_ERR_INVALID_ARG, "state %d: src and dst overlap without being the same", i);
+  return DELS_OK;
 }
 
 }  // namespace
@@ -1337,6 +1424,123 @@ int dels_gather_scaled_rows_bf16(const int64_t* tokens, int64_t tok_stride, int 
       reinterpret_cast<cudaStream_t>(stream), reinterpret_cast<const long long*>(tokens), tok_stride, token_keys,
       reinterpret_cast<const __nv_bfloat16*>(emb), ld_emb, alpha, n_pos, B, r, V,
       reinterpret_cast<__nv_bfloat16*>(s_scaled), reinterpret_cast<long long*>(keys), counter, status));
+  return DELS_OK;
+}
+
+size_t dels_beam_select_workspace_bytes(int n_seq, int beams, int select, int V) {
+  if (n_seq <= 0 || beams <= 0 || select <= 0 || V <= 0) return DELS_WS_HEADER_BYTES;
+  return DELS_WS_HEADER_BYTES + beam_scratch(n_seq, beams, select, V, nullptr, nullptr);
+}
+
+int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const void* base, int64_t ld_base,
+                     const float* prior, const float* beta, const float* cum, const uint8_t* finished, int pad_token,
+                     int n_seq, int beams, int select, int V, int32_t* parents, int64_t* tokens, float* scores,
+                     void* ws, size_t ws_bytes, void* stream) {
+  int rc;
+  if (n_seq < 0) return fail(DELS_ERR_INVALID_ARG, "n_seq must be >= 0 (got %d)", n_seq);
+  if (beams < 1 || beams > kBeamMax || select < 1 || select > kBeamMax)
+    return fail(DELS_ERR_INVALID_ARG, "beams and select must be in 1..%d (got %d, %d)", kBeamMax, beams, select);
+  if (V < select || V > DELS_BEAM_MAX_VOCAB)
+    return fail(DELS_ERR_INVALID_ARG, "V must be in select..%d (got %d, select %d)", DELS_BEAM_MAX_VOCAB, V, select);
+  if ((long long)n_seq * beams > (1ll << 22))
+    return fail(DELS_ERR_INVALID_ARG, "at most 2^22 rows (got %lld)", (long long)n_seq * beams);
+  if (dtype != DELS_DTYPE_BF16 && dtype != DELS_DTYPE_F32) return fail(DELS_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+  const size_t elem = dtype == DELS_DTYPE_BF16 ? 2 : 4;
+  if (n_seq > 0 && (logits == nullptr || cum == nullptr || parents == nullptr || tokens == nullptr || scores == nullptr))
+    return fail(DELS_ERR_INVALID_ARG, "NULL argument");
+  if (ld_logits < V || (base != nullptr && ld_base < V))
+    return fail(DELS_ERR_INVALID_ARG, "leading dimension below V = %d", V);
+  if (prior != nullptr && beta == nullptr) return fail(DELS_ERR_INVALID_ARG, "beta is NULL but prior is given");
+  if (finished != nullptr && (pad_token < 0 || pad_token >= V))
+    return fail(DELS_ERR_INVALID_ARG, "pad_token %d outside the vocabulary of %d", pad_token, V);
+  if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(base)) % elem != 0)
+    return fail(DELS_ERR_ALIGNMENT, "logits and base must be aligned to their elements");
+  WsHeader hdr;
+  if ((rc = ws_header(ws, ws_bytes, dels_beam_select_workspace_bytes(n_seq, beams, select, V), &hdr)) != DELS_OK)
+    return rc;
+  DeviceState* ds = nullptr;
+  if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
+  if (n_seq == 0) return DELS_OK;
+  BeamSelectArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.logits = logits;
+  a.ld = ld_logits;
+  a.base = base;
+  a.ld_base = ld_base;
+  a.prior = prior;
+  a.beta = beta;
+  a.cum = cum;
+  a.finished = finished;
+  a.pad_token = pad_token;
+  a.n_seq = n_seq;
+  a.beams = beams;
+  a.select = select;
+  a.V = V;
+  a.parents = parents;
+  a.tokens = reinterpret_cast<long long*>(tokens);
+  a.scores = scores;
+  beam_scratch(n_seq, beams, select, V, static_cast<char*>(ws) + DELS_WS_HEADER_BYTES, &a);
+  // 16-byte loads need every row to start on a 16-byte boundary
+  const bool vec = aligned16(logits) && (ld_logits * elem) % 16 == 0 &&
+                   (base == nullptr || (aligned16(base) && (ld_base * elem) % 16 == 0)) && aligned16(prior);
+  const bool mix = base != nullptr || prior != nullptr;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == DELS_DTYPE_BF16 ? (mix ? launch_beam_select<__nv_bfloat16, true>(a, vec, st)
+                                         : launch_beam_select<__nv_bfloat16, false>(a, vec, st))
+                                  : (mix ? launch_beam_select<float, true>(a, vec, st)
+                                         : launch_beam_select<float, false>(a, vec, st));
+}
+
+int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t* parents, int n_seq, int beams,
+                      int select, int32_t* status, void* stream) {
+  int rc;
+  if (n_seq < 0 || n_states < 0) return fail(DELS_ERR_INVALID_ARG, "bad counts n_seq=%d n_states=%d", n_seq, n_states);
+  if (beams < 1 || beams > kBeamMax || select < 1 || select > kBeamMax)
+    return fail(DELS_ERR_INVALID_ARG, "beams and select must be in 1..%d (got %d, %d)", kBeamMax, beams, select);
+  if (n_states > 0 && (states == nullptr || (parents == nullptr && n_seq > 0)))
+    return fail(DELS_ERR_INVALID_ARG, "NULL argument");
+  for (int i = 0; i < n_states; ++i)
+    if ((rc = check_beam_state(states[i], i, n_seq, beams, select)) != DELS_OK) return rc;
+  DeviceState* ds = nullptr;
+  if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
+  if (n_seq == 0) return DELS_OK;
+  // the widest piece of a row that all beams' copies of it leave room for in shared memory
+  const int room = kBeamReorderSmem / beams / 16 * 16;
+  for (int first = 0; first < n_states; first += kBeamStatesPerLaunch) {
+    BeamReorderArgs a;
+    std::memset(&a, 0, sizeof(a));
+    for (int i = first; i < n_states && i < first + kBeamStatesPerLaunch; ++i) {
+      const dels_beam_state& d = states[i];
+      if (d.outer == 0 || d.inner_bytes == 0) continue;
+      BeamState& s = a.st[a.n_states++];
+      s.src = static_cast<const char*>(d.src);
+      s.dst = static_cast<char*>(d.dst);
+      s.src_row = d.src_row_stride;
+      s.dst_row = d.dst_row_stride;
+      s.src_outer = d.outer > 1 ? d.src_outer_stride : 0;
+      s.dst_outer = d.outer > 1 ? d.dst_outer_stride : 0;
+      s.outer = (int)d.outer;
+      s.inner = d.inner_bytes;
+      const unsigned long long bits = reinterpret_cast<uintptr_t>(d.src) | reinterpret_cast<uintptr_t>(d.dst) |
+                                      (unsigned long long)(s.src_row | s.dst_row | s.src_outer | s.dst_outer | s.inner);
+      s.width = 16;
+      while (s.width > 1 && bits % s.width != 0) s.width /= 2;
+      s.chunk = (int)(s.inner < room ? (s.inner + 15) / 16 * 16 : room);
+      s.chunks = cdiv(s.inner, s.chunk);
+      s.tile0 = a.tiles;
+      a.tiles += (long long)n_seq * s.outer * s.chunks;
+    }
+    if (a.tiles == 0) continue;
+    a.parents = parents;
+    a.n_seq = n_seq;
+    a.beams = beams;
+    a.select = select;
+    a.status = status;
+    const long long most = 16ll * ds->sm_count;
+    DELS_CHECK_PDL("beam_reorder_kernel launch", launch_pdl(beam_reorder_kernel,
+        dim3((unsigned)(a.tiles < most ? a.tiles : most)), dim3(kBeamThreads), 0,
+        reinterpret_cast<cudaStream_t>(stream), a));
+  }
   return DELS_OK;
 }
 

@@ -859,6 +859,162 @@ def correction_mid_tc(
     return s_scaled
 
 
+# --------------------------------------------------------------------------- beam drafting
+@dataclass
+class BeamOut:
+    parents: torch.Tensor  # int32 [n_seq, select], the beam (0..beams-1) each child extends
+    tokens: torch.Tensor  # int64 [n_seq, select]
+    scores: torch.Tensor  # fp32 [n_seq, select], best first
+
+
+_BEAM_DTYPES = {torch.bfloat16: _lib.DELS_DTYPE_BF16, torch.float32: _lib.DELS_DTYPE_F32}
+
+
+def _require_dense(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
+    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device} "
+                         f"(got {t.dtype} {tuple(t.shape)} on {t.device}, stride {t.stride()})")
+
+
+def beam_select(
+    logits: torch.Tensor,
+    scores: torch.Tensor,
+    *,
+    select: int | None = None,
+    base: torch.Tensor | None = None,
+    prior: torch.Tensor | None = None,
+    beta: torch.Tensor | None = None,
+    finished: torch.Tensor | None = None,
+    pad_token: int = 0,
+    out: BeamOut | None = None,
+    ws: Workspace | None = None,
+) -> BeamOut:
+    """The ``select`` best extensions (default: as many as there are beams) of every
+    sequence's beams by one token, best first.
+
+    ``logits`` [n_seq * beams, V] (bf16 or fp32) and ``scores`` [n_seq, beams] (fp32, the
+    beams' accumulated log-probabilities); a candidate scores its beam's score plus
+    log_softmax(x)[token] of x = logits, or, with ``base`` [n_seq, V] (draft logits the
+    beams of a sequence share) and ``prior`` [V] with ``beta`` [1],
+    x = (base + logits) - beta * prior.  Equal scores: the lower beam, then the larger x,
+    then the lower token.  A beam whose ``finished`` [n_seq, beams] (bool) is set goes on
+    only with ``pad_token`` at its score, and its logits are not read.  Masked tokens hold
+    -inf or the type's lowest value; a row may be masked whole.  ``out.scores`` may be
+    ``scores`` itself when ``select`` equals the beams."""
+    if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda" or logits.dim() != 2 \
+            or logits.dtype not in _BEAM_DTYPES:
+        raise ValueError("logits must be a 2-D bf16 or fp32 CUDA tensor; there is no CPU path")
+    dev, dtype = logits.device, logits.dtype
+    rows, V = logits.shape
+    if scores.dim() != 2:
+        raise ValueError(f"scores must be [n_seq, beams] (got {tuple(scores.shape)})")
+    n_seq, beams = scores.shape
+    n = beams if select is None else int(select)
+    if rows != n_seq * beams:
+        raise ValueError(f"logits {tuple(logits.shape)} do not match scores {tuple(scores.shape)}")
+    _require_dense("scores", scores, torch.float32, (n_seq, beams), dev)
+    if base is not None and (base.dtype != dtype or base.shape != (n_seq, V) or base.device != dev):
+        raise ValueError(f"base must be {dtype} {(n_seq, V)} on {dev} (got {base.dtype} {tuple(base.shape)})")
+    if prior is not None:
+        _require_dense("prior", prior, torch.float32, (V,), dev)
+        if beta is None:
+            raise ValueError("prior needs beta")
+        _require_dense("beta", beta, torch.float32, (1,), dev)
+    if finished is not None:
+        if finished.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"finished must be bool or uint8 (got {finished.dtype})")
+        _require_dense("finished", finished, finished.dtype, (n_seq, beams), dev)
+    if out is None:
+        out = BeamOut(torch.empty(n_seq, n, dtype=torch.int32, device=dev),
+                      torch.empty(n_seq, n, dtype=torch.int64, device=dev),
+                      torch.empty(n_seq, n, dtype=torch.float32, device=dev))
+    else:
+        _require_dense("out.parents", out.parents, torch.int32, (n_seq, n), dev)
+        _require_dense("out.tokens", out.tokens, torch.int64, (n_seq, n), dev)
+        _require_dense("out.scores", out.scores, torch.float32, (n_seq, n), dev)
+    need = _lib.query("dels_beam_select_workspace_bytes", n_seq, beams, n, V)
+    ws = workspace(need, dev) if ws is None else ws.ensure(need)
+    _lib.call(
+        "dels_beam_select", _ptr(logits), _BEAM_DTYPES[dtype], _row_major("logits", logits), _ptr(base),
+        0 if base is None else _row_major("base", base), _ptr(prior), _ptr(beta), _ptr(scores), _ptr(finished),
+        int(pad_token), n_seq, beams, n, V, _ptr(out.parents), _ptr(out.tokens), _ptr(out.scores), ws.ptr, ws.nbytes,
+        _stream(dev),
+    )
+    return out
+
+
+def beam_select_workspace_bytes(n_seq: int, beams: int, select: int, V: int) -> int:
+    return int(_lib.query("dels_beam_select_workspace_bytes", n_seq, beams, select, V))
+
+
+def _beam_state(i: int, src: torch.Tensor, dst: torch.Tensor) -> tuple:
+    """The dels_beam_state of one (src, dst) pair: rows of ``outer`` runs of contiguous bytes."""
+    item = src.element_size()
+    if src.is_contiguous() and dst.is_contiguous():
+        inner = 1
+        for n in src.shape[1:]:
+            inner *= n
+        return src.data_ptr(), dst.data_ptr(), inner * item, inner * item, 0, 0, 1, inner * item
+    shape, ss, ds = src.shape, src.stride(), dst.stride()
+    inner, k = 1, src.dim() - 1
+    while k >= 1 and (shape[k] == 1 or (ss[k] == inner and ds[k] == inner)):
+        inner *= shape[k]
+        k -= 1
+    outer, so, do = 1, 0, 0
+    for j in range(k, 0, -1):
+        if shape[j] == 1:
+            continue
+        if outer == 1:
+            so, do = ss[j], ds[j]
+        elif ss[j] != so * outer or ds[j] != do * outer:
+            raise ValueError(f"state {i}: rows of shape {tuple(shape[1:])} must be evenly spaced runs of contiguous "
+                             f"elements (strides {ss}, {ds})")
+        outer *= shape[j]
+    return (src.data_ptr(), dst.data_ptr(), ss[0] * item, ds[0] * item, so * item, do * item, outer, inner * item)
+
+
+def beam_reorder(
+    states: list[torch.Tensor],
+    parents: torch.Tensor,
+    *,
+    beams: int,
+    out: list[torch.Tensor] | None = None,
+    status: torch.Tensor | None = None,
+) -> list[torch.Tensor]:
+    """Move every state's rows after a selection: out[b * select + j] =
+    state[b * beams + parents[b, j]].
+
+    ``states`` are CUDA tensors of any type whose first dimension is n_seq * beams (GRU
+    states, token histories, caches cut to their used length); ``parents`` is
+    ``beam_select``'s int32 [n_seq, select].  ``out`` gives the destinations ([n_seq *
+    select, ...]); ``out=states`` reorders in place (select == beams).  The tensors must not
+    overlap otherwise.  A parent outside 0..beams-1 leaves its child's row as it was and
+    stores an error code in ``status`` (int32 [1], zero before)."""
+    _require_cuda("parents", parents, torch.int32, 2)
+    dev = parents.device
+    n_seq, n = parents.shape
+    _require_dense("parents", parents, torch.int32, (n_seq, n), dev)
+    if status is not None:
+        _require_dense("status", status, torch.int32, (1,), dev)
+    rows = n_seq * int(beams)
+    if out is None:
+        out = [torch.empty((n_seq * n, *t.shape[1:]), dtype=t.dtype, device=dev) for t in states]
+    if len(out) != len(states):
+        raise ValueError(f"{len(states)} states, but {len(out)} outputs")
+    table: list[int] = []
+    for i, (src, dst) in enumerate(zip(states, out)):
+        if src.device != dev or dst.device != dev:
+            raise ValueError(f"state {i}: {src.device} -> {dst.device}, but parents are on {dev}")
+        if src.dim() < 1 or src.shape[0] != rows or dst.dtype != src.dtype or dst.shape[0] != n_seq * n \
+                or dst.shape[1:] != src.shape[1:]:
+            raise ValueError(f"state {i}: {src.dtype} {tuple(src.shape)} -> {dst.dtype} {tuple(dst.shape)} does not "
+                             f"match {n_seq} sequences of {beams} -> {n} beams")
+        table.extend(_beam_state(i, src, dst))
+    _lib.call("dels_beam_reorder", (ctypes.c_int64 * len(table))(*table), len(states), _ptr(parents), n_seq,
+              int(beams), n, _ptr(status), _stream(dev))
+    return out
+
+
 def zero_pad(t: torch.Tensor | None, rows: int | None = None, cols: int | None = None) -> torch.Tensor | None:
     """``t`` zero-padded to ``rows`` (dim 0) x ``cols`` (dim 1).  The runners carry weight
     widths as multiples of 8 because TMA tiles need 16-byte row pitches; the zero entries

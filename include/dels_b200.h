@@ -341,6 +341,57 @@ DELS_API int dels_correction_mid_tc_bf16(const void* h, int64_t ld_h, const void
                                          int64_t* keys, void* ws, size_t ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
+ * Beam drafting (no counterpart in the reference, which drafts one chain per sequence):
+ * a sequence keeps `beams` candidate chains, each step extends every chain by every
+ * token, and the best `select` of these candidates go on.
+ * --------------------------------------------------------------------------------- */
+#define DELS_DTYPE_BF16 0
+#define DELS_DTYPE_F32 1
+#define DELS_BEAM_MAX 64          /* beams and select are at most this */
+#define DELS_BEAM_MAX_VOCAB 524288
+
+/* Selection.  Row i = b * beams + k is beam k of sequence b, with logits
+ *   x[v] = logits[i, v]                                   or, with base and / or prior,
+ *   x[v] = (base[b, v] + logits[i, v]) - beta[0] * prior[v]   (fp32, each operation rounded)
+ * and a candidate (k, v) scores cum[i] + log_softmax(x)[v], computed in fp32 as
+ * (x[v] - max x) + (cum[i] - log sum exp(x - max x)).  The `select` best candidates of
+ * each sequence, best first: the higher score, then the lower beam, then the larger x,
+ * then the lower token.  A token at -inf scores -inf (a row may hold nothing else); a NaN
+ * score is above every other.  A beam with finished[i] != 0 has one candidate, pad_token
+ * at score cum[i] (its other tokens score -inf), and its logits are not read.
+ *   logits [n_seq * beams, V] and base [n_seq, V]: bf16 or fp32 (dtype), row strides
+ *   ld_logits / ld_base, any alignment of whole elements; prior [V] fp32; beta [1];
+ *   cum [n_seq, beams] fp32; finished bytes [n_seq, beams] or NULL.
+ *   parents [n_seq, select] int32 (0..beams-1), tokens [n_seq, select] int64, scores
+ *   [n_seq, select] fp32, which may be `cum` itself when select == beams.
+ * 1 <= beams, select <= DELS_BEAM_MAX, select <= V <= DELS_BEAM_MAX_VOCAB;
+ * ws >= dels_beam_select_workspace_bytes(). */
+DELS_API size_t dels_beam_select_workspace_bytes(int n_seq, int beams, int select, int V);
+DELS_API int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const void* base, int64_t ld_base,
+                              const float* prior, const float* beta, const float* cum, const uint8_t* finished,
+                              int pad_token, int n_seq, int beams, int select, int V, int32_t* parents,
+                              int64_t* tokens, float* scores, void* ws, size_t ws_bytes, void* stream);
+
+/* Reordering of the beams' states after a selection: for every state and sequence b,
+ *   dst[b * select + j] = src[b * beams + parents[b, j]],  j < select.
+ * A state's row is `outer` runs of `inner_bytes` contiguous bytes (a cache cut to its used
+ * length); strides are in bytes.  src == dst with equal strides reorders in place
+ * (select == beams); any other overlap of the two memory spans is refused.  The states of
+ * one call must not overlap each other.  A parent outside 0..beams-1 leaves its child's
+ * rows as they were and stores DELS_ERR_INVALID_ARG in *status (an int32 in device memory,
+ * zero before, or NULL). */
+typedef struct dels_beam_state {
+  const void* src;
+  void* dst;
+  int64_t src_row_stride, dst_row_stride;
+  int64_t src_outer_stride, dst_outer_stride;
+  int64_t outer;
+  int64_t inner_bytes;
+} dels_beam_state;
+DELS_API int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t* parents, int n_seq,
+                               int beams, int select, int32_t* status, void* stream);
+
+/* ---------------------------------------------------------------------------------
  * Allocation-free variant of dels_draft_score_bf16 (no counterpart in the reference).
  * For callers that cannot hand the library device memory — an FFI host without a
  * device allocator, or a serving engine whose memory pool already owns the device —
