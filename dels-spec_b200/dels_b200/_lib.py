@@ -26,6 +26,7 @@ DELS_ACT_SILU = 1
 DELS_FLAG_KEYS_READY = 1
 DELS_DTYPE_BF16 = 0
 DELS_DTYPE_F32 = 1
+DELS_I8_MAX_K = 131071
 DELS_BEAM_MAX = 64
 DELS_BEAM_MAX_VOCAB = 524288
 DELS_WS_HEADER_BYTES = 256
@@ -96,6 +97,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dels_linear_bf16": (_I, [_P, _I64, _P, _I64, _P, _I, _I, _I, _P, _I64, _P, _SZ, _P]),
     "dels_correction_mid_bf16": (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P, _P, _P]),
     "dels_correction_mid_tc_bf16": (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _P, _P, _P, _P, _SZ, _P]),
+    "dels_quantize_rows_i8": (_I, [_P, _I, _I64, _I, _I, _P, _I64, _P, _P]),
+    "dels_linear_i8": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _I, _I, _I, _P, _I, _I64, _P, _SZ, _P]),
+    "dels_linear_w8a8_workspace_bytes": (_SZ, [_I, _I]),
+    "dels_linear_w8a8": (_I, [_P, _I, _I64, _P, _I64, _P, _P, _I, _I, _I, _P, _I, _I64, _P, _SZ, _P]),
     "dels_beam_select_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "dels_beam_select": (
         _I,

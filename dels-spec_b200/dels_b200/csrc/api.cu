@@ -13,6 +13,7 @@
 
 #include "beam_kernels.cuh"
 #include "f32_score.cuh"
+#include "i8_gemm.cuh"
 #include "runner_kernels.cuh"
 #include "small_kernels.cuh"
 #include "tc_gemm.cuh"
@@ -166,6 +167,22 @@ int make_map_base_bf16(CUtensorMap* m, const void* ptr, long long n, long long r
   return DELS_OK;
 }
 
+// 2-D int8 tensor map over a row-major [outer, inner] matrix with leading dimension `ld`
+// bytes, box = [box_outer rows, 128 elements], 128-byte swizzle, zero fill outside.
+int make_map_i8(CUtensorMap* m, const void* ptr, long long inner, long long outer, long long ld, int box_outer) {
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)kI8BK, (cuuint32_t)box_outer};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(DELS_ERR_CUDA, "cuTensorMapEncodeTiled (int8) failed (%d) for [%lld x %lld], ld %lld", (int)r, outer,
+                inner, ld);
+  return DELS_OK;
+}
+
 int make_map_vec_f32(CUtensorMap* m, const float* ptr, long long n, int box_n) {
   // one row of n; the row stride is never stepped but must be a multiple of 16 bytes
   cuuint64_t dims[2] = {(cuuint64_t)n, 1};
@@ -276,6 +293,20 @@ int init_device(int dev) {
     SET((beam_row_kernel<__nv_bfloat16, true>), kBeamRowSmemMax);
     SET(beam_merge_kernel, kBeamMax * kBeamMax * (int)sizeof(uint32_t));
     SET(beam_reorder_kernel, 0);
+    SET((i8_gemm_kernel<16, __nv_bfloat16>), I8Config<16>::kSmemBytes);
+    SET((i8_gemm_kernel<32, __nv_bfloat16>), I8Config<32>::kSmemBytes);
+    SET((i8_gemm_kernel<64, __nv_bfloat16>), I8Config<64>::kSmemBytes);
+    SET((i8_gemm_kernel<128, __nv_bfloat16>), I8Config<128>::kSmemBytes);
+    SET((i8_gemm_kernel<256, __nv_bfloat16>), I8Config<256>::kSmemBytes);
+    SET((i8_gemm_kernel<16, float>), I8Config<16>::kSmemBytes);
+    SET((i8_gemm_kernel<32, float>), I8Config<32>::kSmemBytes);
+    SET((i8_gemm_kernel<64, float>), I8Config<64>::kSmemBytes);
+    SET((i8_gemm_kernel<128, float>), I8Config<128>::kSmemBytes);
+    SET((i8_gemm_kernel<256, float>), I8Config<256>::kSmemBytes);
+    SET((quantize_rows_kernel<float, false>), 0);
+    SET((quantize_rows_kernel<float, true>), 0);
+    SET((quantize_rows_kernel<__nv_bfloat16, false>), 0);
+    SET((quantize_rows_kernel<__nv_bfloat16, true>), 0);
 #undef SET
   }
   if (rc == DELS_OK) {
@@ -758,6 +789,112 @@ int check_beam_state(const dels_beam_state& d, int i, int n_seq, int beams, int 
   if (s0 < d1 && d0 < s1) return fail(DELS_ERR_INVALID_ARG, "state %d: src and dst overlap without being the same", i);
   return DELS_OK;
 }
+
+// ------------------------------------------------------------------ 8-bit product
+int check_i8_matrix(const char* name, const void* p, long long ld, long long k) {
+  if (p == nullptr) return fail(DELS_ERR_INVALID_ARG, "%s is NULL", name);
+  if (!aligned16(p)) return fail(DELS_ERR_ALIGNMENT, "%s must be 16-byte aligned", name);
+  if (ld < k || (ld % 16) != 0)
+    return fail(DELS_ERR_ALIGNMENT, "%s: leading dimension %lld must be >= %lld and a multiple of 16", name, ld, k);
+  return DELS_OK;
+}
+
+int check_i8_shape(int rows, int K, int N) {
+  if (rows < 0 || K <= 0 || N <= 0) return fail(DELS_ERR_INVALID_ARG, "bad shape rows=%d K=%d N=%d", rows, K, N);
+  if (K > DELS_I8_MAX_K)
+    return fail(DELS_ERR_UNSUPPORTED, "K = %d: sums of more than %d products leave 32 bits", K, DELS_I8_MAX_K);
+  return DELS_OK;
+}
+
+int launch_quantize_rows(const void* x, int dtype, long long ld_x, int rows, int K, int8_t* q, long long ld_q,
+                         float* scale, int sm_count, cudaStream_t st) {
+  const int grid = rows < 8 * sm_count ? rows : 8 * sm_count;
+  const bool vec = aligned16(x) && (ld_x * (dtype == DELS_DTYPE_BF16 ? 2 : 4)) % 16 == 0;
+  if (dtype == DELS_DTYPE_BF16) {
+    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(x);
+    DELS_CHECK_PDL("quantize_rows_kernel launch",
+                   launch_pdl(vec ? quantize_rows_kernel<__nv_bfloat16, true> : quantize_rows_kernel<__nv_bfloat16, false>,
+                              dim3(grid), dim3(kQuantThreads), 0, st, p, ld_x, rows, K, q, ld_q, scale));
+  } else {
+    const float* p = static_cast<const float*>(x);
+    DELS_CHECK_PDL("quantize_rows_kernel launch",
+                   launch_pdl(vec ? quantize_rows_kernel<float, true> : quantize_rows_kernel<float, false>, dim3(grid),
+                              dim3(kQuantThreads), 0, st, p, ld_x, rows, K, q, ld_q, scale));
+  }
+  return DELS_OK;
+}
+
+template <int TN, typename OutT>
+int launch_i8_tn(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, I8Args a, int sm_count,
+                 cudaStream_t st) {
+  int rc = ensure_encode();
+  if (rc != DELS_OK) return rc;
+  a.m_tiles = cdiv(a.rows, TN);
+  // Channels a weight tile loads: the height whose waves take the shortest.  A block of K
+  // costs its bytes or its MMAs (128 lanes run however few are loaded: about as long as
+  // TN / 2 channels take to load), and a hand-off worth about 32 channels.
+  long long best = -1;
+  for (int box = 8; box <= kBM; box += 8) {
+    const long long units = (long long)cdiv(a.n_out, box) * a.m_tiles;
+    const long long cost = (long long)cdiv(units, sm_count) * (32 + (box > TN / 2 ? box : TN / 2));
+    if (best < 0 || cost <= best) {
+      best = cost;
+      a.box = box;
+    }
+  }
+  a.n_tiles = cdiv(a.n_out, a.box);
+  a.kb = cdiv(K, kI8BK);
+  CUtensorMap mw, mx;
+  if ((rc = make_map_i8(&mw, wq, K, a.n_out, ld_w, a.box)) != DELS_OK) return rc;
+  if ((rc = make_map_i8(&mx, xq, K, a.rows, ld_x, TN)) != DELS_OK) return rc;
+  const long long units = (long long)a.n_tiles * a.m_tiles;
+  DELS_CHECK_PDL("i8_gemm_kernel launch",
+                 launch_pdl(i8_gemm_kernel<TN, OutT>, dim3((unsigned)(units < sm_count ? units : sm_count)),
+                            dim3(kTcThreads), I8Config<TN>::kSmemBytes, st, mw, mx, a));
+  return DELS_OK;
+}
+
+template <typename OutT>
+int launch_i8_out(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, const I8Args& a, int sm_count,
+                  cudaStream_t st) {
+  if (a.rows <= 16) return launch_i8_tn<16, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
+  if (a.rows <= 32) return launch_i8_tn<32, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
+  if (a.rows <= 64) return launch_i8_tn<64, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
+  if (a.rows <= 128) return launch_i8_tn<128, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
+  return launch_i8_tn<256, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
+}
+
+int check_i8_out(const void* out, int out_dtype, long long ld_out, const void* bias, int N) {
+  if (out_dtype != DELS_DTYPE_BF16 && out_dtype != DELS_DTYPE_F32)
+    return fail(DELS_ERR_INVALID_ARG, "unknown dtype %d", out_dtype);
+  const size_t elem = out_dtype == DELS_DTYPE_BF16 ? 2 : 4;
+  if (out == nullptr || ld_out < N) return fail(DELS_ERR_INVALID_ARG, "out is NULL or ld_out < N");
+  if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(bias)) % elem != 0)
+    return fail(DELS_ERR_ALIGNMENT, "out and bias must be aligned to their elements");
+  return DELS_OK;
+}
+
+int launch_i8(const void* xq, long long ld_x, const float* x_scale, const void* wq, long long ld_w,
+              const float* w_scale, const void* bias, int rows, int K, int N, void* out, int out_dtype,
+              long long ld_out, bool early, int* status, int sm_count, cudaStream_t st) {
+  I8Args a;
+  std::memset(&a, 0, sizeof(a));
+  a.rows = rows;
+  a.n_out = N;
+  a.sx = x_scale;
+  a.sw = w_scale;
+  a.bias = bias;
+  a.out = out;
+  a.ld_out = ld_out;
+  a.store2 = N % 2 == 0 && ld_out % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
+  a.early = early && g_use_pdl;
+  a.status = status;
+  return out_dtype == DELS_DTYPE_BF16 ? launch_i8_out<__nv_bfloat16>(xq, ld_x, wq, ld_w, K, a, sm_count, st)
+                                      : launch_i8_out<float>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
+}
+
+// Row stride of the quantised rows that a fused call keeps in its workspace.
+long long i8_padded(int K) { return ((long long)K + 15) / 16 * 16; }
 
 }  // namespace
 
@@ -1542,6 +1679,71 @@ int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t
         reinterpret_cast<cudaStream_t>(stream), a));
   }
   return DELS_OK;
+}
+
+int dels_quantize_rows_i8(const void* x, int dtype, int64_t ld_x, int rows, int K, int8_t* q, int64_t ld_q,
+                          float* scale, void* stream) {
+  int rc;
+  if (rows < 0 || K <= 0) return fail(DELS_ERR_INVALID_ARG, "bad shape rows=%d K=%d", rows, K);
+  if (dtype != DELS_DTYPE_BF16 && dtype != DELS_DTYPE_F32) return fail(DELS_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+  if (rows > 0 && (x == nullptr || scale == nullptr)) return fail(DELS_ERR_INVALID_ARG, "NULL argument");
+  if (ld_x < K) return fail(DELS_ERR_INVALID_ARG, "ld_x %lld < K %d", (long long)ld_x, K);
+  if (reinterpret_cast<uintptr_t>(x) % (dtype == DELS_DTYPE_BF16 ? 2 : 4) != 0)
+    return fail(DELS_ERR_ALIGNMENT, "x must be aligned to its elements");
+  if (rows > 0 && (rc = check_i8_matrix("q", q, ld_q, K)) != DELS_OK) return rc;
+  DeviceState* ds = nullptr;
+  if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
+  if (rows == 0) return DELS_OK;
+  return launch_quantize_rows(x, dtype, ld_x, rows, K, q, ld_q, scale, ds->sm_count,
+                              reinterpret_cast<cudaStream_t>(stream));
+}
+
+int dels_linear_i8(const int8_t* xq, int64_t ld_xq, const float* x_scale, const int8_t* wq, int64_t ld_wq,
+                   const float* w_scale, const void* bias, int rows, int K, int N, void* out, int out_dtype,
+                   int64_t ld_out, void* ws, size_t ws_bytes, void* stream) {
+  int rc;
+  if ((rc = check_i8_shape(rows, K, N)) != DELS_OK) return rc;
+  if (rows > 0) {
+    if ((rc = check_i8_matrix("xq", xq, ld_xq, K)) != DELS_OK) return rc;
+    if ((rc = check_i8_out(out, out_dtype, ld_out, bias, N)) != DELS_OK) return rc;
+    if (x_scale == nullptr) return fail(DELS_ERR_INVALID_ARG, "x_scale is NULL");
+  }
+  if ((rc = check_i8_matrix("wq", wq, ld_wq, K)) != DELS_OK) return rc;
+  if (w_scale == nullptr) return fail(DELS_ERR_INVALID_ARG, "w_scale is NULL");
+  WsHeader hdr;
+  if ((rc = ws_header(ws, ws_bytes, DELS_WS_HEADER_BYTES, &hdr)) != DELS_OK) return rc;
+  DeviceState* ds = nullptr;
+  if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
+  if (rows == 0) return DELS_OK;
+  // the kernel before this one may be the one that quantised the weights
+  return launch_i8(xq, ld_xq, x_scale, wq, ld_wq, w_scale, bias, rows, K, N, out, out_dtype, ld_out, false, hdr.status,
+                   ds->sm_count, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t dels_linear_w8a8_workspace_bytes(int rows, int K) {
+  if (rows <= 0 || K <= 0) return DELS_WS_HEADER_BYTES;
+  return DELS_WS_HEADER_BYTES + align256((size_t)rows * sizeof(float)) + align256((size_t)rows * i8_padded(K));
+}
+
+int dels_linear_w8a8(const void* x, int x_dtype, int64_t ld_x, const int8_t* wq, int64_t ld_wq, const float* w_scale,
+                     const void* bias, int rows, int K, int N, void* out, int out_dtype, int64_t ld_out, void* ws,
+                     size_t ws_bytes, void* stream) {
+  int rc;
+  if ((rc = check_i8_shape(rows, K, N)) != DELS_OK) return rc;
+  if (rows > 0 && (rc = check_i8_out(out, out_dtype, ld_out, bias, N)) != DELS_OK) return rc;
+  if ((rc = check_i8_matrix("wq", wq, ld_wq, K)) != DELS_OK) return rc;
+  if (w_scale == nullptr) return fail(DELS_ERR_INVALID_ARG, "w_scale is NULL");
+  WsHeader hdr;
+  if ((rc = ws_header(ws, ws_bytes, dels_linear_w8a8_workspace_bytes(rows, K), &hdr)) != DELS_OK) return rc;
+  DeviceState* ds = nullptr;
+  if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
+  char* body = static_cast<char*>(ws) + DELS_WS_HEADER_BYTES;
+  float* x_scale = reinterpret_cast<float*>(body);
+  int8_t* xq = reinterpret_cast<int8_t*>(body + align256((size_t)rows * sizeof(float)));
+  if ((rc = dels_quantize_rows_i8(x, x_dtype, ld_x, rows, K, xq, i8_padded(K), x_scale, stream)) != DELS_OK) return rc;
+  if (rows == 0) return DELS_OK;
+  return launch_i8(xq, i8_padded(K), x_scale, wq, ld_wq, w_scale, bias, rows, K, N, out, out_dtype, ld_out, true,
+                   hdr.status, ds->sm_count, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,333 @@
+// 8-bit integer product with a scale for each row and each channel (sm_100a).
+//
+//   y[m, n] = (sum_k xq[m, k] wq[n, k]) * sx[m] * sw[n] (+ bias[n])
+//
+// xq [rows, K], wq [n_out, K] int8, K-major; the sum is exact in the tensor cores' 32-bit
+// integers (tcgen05 kind::i8), so no order of additions shows in the result.
+//
+// The weights are the MMA's M side (128 TMEM lanes, one channel each) and the rows its N
+// side (TN columns), whatever the number of rows: a weight-streaming call of a few rows
+// loads 128 channels for every TN = 16 rows, and a large call runs full 128 x 256 tiles.
+// K goes in blocks of 128 (one 128-byte swizzled line of every operand row), staged by TMA
+// in a ring; two accumulators in TMEM let a tile's epilogue overlap the next one's MMAs.
+//
+// Warp roles (192 threads): warp 0 = TMA producer, warp 1 = TMEM allocator + MMA issuer,
+// warps 2..5 = epilogue (one thread per channel).
+#pragma once
+
+#include "tc_gemm.cuh"
+
+namespace dels {
+
+constexpr int kI8BK = 128;  // K elements (bytes) of a block
+
+struct I8Args {
+  int rows, n_out, kb;     // kb: blocks of K
+  int box;                 // channels a weight tile loads (<= 128; the MMA always runs 128 lanes)
+  int n_tiles, m_tiles;    // weight tiles, row tiles
+  const float* sx;         // [rows]
+  const float* sw;         // [n_out]
+  const void* bias;        // [n_out] of the output's type, or null
+  void* out;               // [rows, n_out] bf16 or fp32
+  long long ld_out;
+  int store2;              // bf16: two channels per store (even ld_out, 4-byte aligned out)
+  int early;               // the weights are not written by the previous kernel: load them before waiting for it
+  int* status;
+};
+
+template <int TN>
+struct I8Config {
+  static constexpr int kABytes = kBM * kI8BK;
+  static constexpr int kBBytes = TN * kI8BK;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = TN <= 32 ? 10 : (TN == 64 ? 8 : (TN == 128 ? 6 : 4));
+  static constexpr int kTmemCols = 2 * TN <= 32 ? 32 : 2 * TN;
+  static constexpr int kScaleOffset = kStages * kStageBytes;  // [4 warps][TN] row scales
+  static constexpr int kBarOffset = kScaleOffset + 4 * TN * 4;
+  static constexpr int kNumBars = 2 * kStages + 4;
+  static constexpr int kSmemBytes = kBarOffset + kNumBars * 8 + 16 + 1024;
+  static_assert(TN >= 16 && TN <= 256 && (TN & (TN - 1)) == 0, "TN is a power of two in [16, 256]");
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
+// D[tmem] (+)= A[smem] * B[smem]^T, signed 8-bit inputs, 32-bit integer accumulator.
+__device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor of tcgen05.mma kind::i8: signed A and B (both K-major), s32
+// accumulator, shape M x N.
+__host__ __device__ constexpr uint32_t make_idesc_s8_s32(int M, int N) {
+  return (2u << 4)                        // accumulator format: s32
+         | (1u << 7)                      // A format: signed
+         | (1u << 10)                     // B format: signed
+         | ((uint32_t)(N >> 3) << 17)     // N / 8
+         | ((uint32_t)(M >> 4) << 24);    // M / 16
+}
+
+// One channel's results for the COLS rows row0.. of a tile (`valid` of them exist).
+template <int COLS, typename OutT>
+__device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float* scale, float sw, float bias, int valid,
+                                         bool channel_ok, OutT* out, long long ld, bool store2, int lane) {
+  if constexpr (sizeof(OutT) == 2) {
+    if (store2) {
+      // lanes 2i and 2i + 1 swap halves of a pair of rows, so each stores two neighbouring
+      // channels of one row with one 4-byte store
+      const bool odd = lane & 1;
+#pragma unroll
+      for (int j = 0; j < COLS; j += 2) {
+        if (j >= valid) break;
+        const float y0 = __int2float_rn((int)v[j]) * scale[j] * sw + bias;
+        const float y1 = __int2float_rn((int)v[j + 1]) * scale[j + 1] * sw + bias;
+        const float other = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 1);
+        const uint32_t pair = odd ? pack_bf16x2(other, y1) : pack_bf16x2(y0, other);
+        if (channel_ok && j + (int)odd < valid)
+          *reinterpret_cast<uint32_t*>(out + (long long)(j + (int)odd) * ld - (int)odd) = pair;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < COLS; ++j) {
+    if (j >= valid) break;
+    const float y = __int2float_rn((int)v[j]) * scale[j] * sw + bias;
+    if (channel_ok) {
+      if constexpr (sizeof(OutT) == 2)
+        out[j * ld] = __float2bfloat16_rn(y);
+      else
+        out[j * ld] = y;
+    }
+  }
+}
+
+template <int TN, typename OutT>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    i8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                   const I8Args args) {
+  using Cfg = I8Config<TN>;
+  constexpr int S = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base_addr = (raw_addr + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base_addr - raw_addr);
+  const uint32_t a_base = base_addr;
+  const uint32_t b_base = base_addr + S * Cfg::kABytes;
+  float* scales = reinterpret_cast<float*>(smem + Cfg::kScaleOffset);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  auto full_bar = [&](int s) { return smem_u32(&bars[s]); };
+  auto empty_bar = [&](int s) { return smem_u32(&bars[S + s]); };
+  auto tfull_bar = [&](int a) { return smem_u32(&bars[2 * S + a]); };
+  auto tempty_bar = [&](int a) { return smem_u32(&bars[2 * S + 2 + a]); };
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), 4);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_map(&map_w);
+    tma_prefetch_map(&map_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int units = args.n_tiles * args.m_tiles;  // row tiles of one weight tile next to each other
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    if (lane == 0) {
+      const uint32_t tx = (uint32_t)(args.box * kI8BK + Cfg::kBBytes);
+      // The ring's first weight tiles do not depend on the kernel that makes xq.
+      int ahead = 0;
+      if (args.early) {
+        int u = blockIdx.x, kb = 0;
+        while (ahead < S && u < units) {
+          mbar_arrive_expect_tx(full_bar(ahead), tx);
+          tma_load_2d(a_base + ahead * Cfg::kABytes, &map_w, full_bar(ahead), kb * kI8BK, u / args.m_tiles * args.box);
+          ++ahead;
+          if (++kb == args.kb) kb = 0, u += gridDim.x;
+        }
+      }
+      pdl_wait();
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const int n0 = u / args.m_tiles * args.box, m0 = u % args.m_tiles * TN;
+        for (int kb = 0; kb < args.kb; ++kb) {
+          if (issued >= ahead) {
+            if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, args.status)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(full_bar(stage), tx);
+            tma_load_2d(a_base + stage * Cfg::kABytes, &map_w, full_bar(stage), kb * kI8BK, n0);
+          }
+          tma_load_2d(b_base + stage * Cfg::kBBytes, &map_x, full_bar(stage), kb * kI8BK, m0);
+          ++issued;
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        // Aborting: let the copies already in flight land before the CTA exits.
+        const int outstanding = issued < S ? issued : S;
+        for (int i = 0; i < outstanding; ++i) {
+          if (--stage < 0) {
+            stage = S - 1;
+            phase ^= 1u;
+          }
+          const unsigned long long t0 = globaltimer_ns();
+          while (!mbar_try_wait(full_bar(stage), phase) && globaltimer_ns() - t0 < kWaitLimitNs / 20) {
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc_s8_s32(kBM, TN);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, args.status)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * TN);
+        for (int kb = 0; kb < args.kb; ++kb) {
+          if (!mbar_wait(full_bar(stage), phase, abort_flag, args.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t adesc = make_sw128_desc(a_base + stage * Cfg::kABytes);
+          const uint64_t bdesc = make_sw128_desc(b_base + stage * Cfg::kBBytes);
+#pragma unroll
+          for (int k = 0; k < kI8BK / 32; ++k)  // +32 bytes per K step inside the 128-byte swizzled line
+            tc_mma_i8(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          tc_commit(empty_bar(stage));
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        tc_commit(tfull_bar(acc));
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      // Aborting: wait until every MMA issued has completed before TMEM is released.
+      if (!ok || *abort_flag) {
+        const uint32_t drain = tfull_bar(acc);
+        tc_commit(drain);
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, acc_phase) && globaltimer_ns() - t0 < kWaitLimitNs / 20) {
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue
+    pdl_wait();  // sx is another kernel's, and out may be in its hands
+    const int quad = warp & 3;  // TMEM lanes this warp can read
+    float* scale = scales + quad * TN;
+    OutT* out = static_cast<OutT*>(args.out);
+    const OutT* bias_v = static_cast<const OutT*>(args.bias);
+    int acc = 0, scale_m = -1;
+    uint32_t acc_phase = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const int m_tile = u % args.m_tiles, m0 = m_tile * TN;
+      const int in_tile = quad * 32 + lane;
+      const int n = u / args.m_tiles * args.box + in_tile;
+      const bool channel_ok = in_tile < args.box && n < args.n_out;
+      const bool warp_ok = quad * 32 < args.box && n - lane < args.n_out;
+      const int valid = min(TN, args.rows - m0);
+      if (m_tile != scale_m) {
+        __syncwarp();
+        for (int j = lane; j < TN; j += 32) scale[j] = m0 + j < args.rows ? __ldg(args.sx + m0 + j) : 0.0f;
+        __syncwarp();
+        scale_m = m_tile;
+      }
+      const float sw = channel_ok ? __ldg(args.sw + n) : 0.0f;
+      float bias = 0.0f;
+      if (channel_ok && bias_v != nullptr) {
+        if constexpr (sizeof(OutT) == 2)
+          bias = __bfloat162float(bias_v[n]);
+        else
+          bias = bias_v[n];
+      }
+      if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, args.status)) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * TN);
+      OutT* dst = out + (long long)m0 * args.ld_out + n;
+      if (warp_ok) {
+        if constexpr (TN == 16) {
+          uint32_t v[16];
+          tmem_ld_16cols(t_row, v);
+          tmem_ld_wait(v);
+          i8_store<16, OutT>(v, scale, sw, bias, valid, channel_ok, dst, args.ld_out, args.store2 != 0, lane);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < TN && c < valid; c += 32) {
+            uint32_t v[32];
+            tmem_ld_32cols(t_row + (uint32_t)c, v);
+            tmem_ld_wait(v);
+            i8_store<32, OutT>(v, scale + c, sw, bias, valid - c, channel_ok, dst + (long long)c * args.ld_out,
+                               args.ld_out, args.store2 != 0, lane);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty_bar(acc));
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, Cfg::kTmemCols);
+  }
+}
+
+// Rows to 8 bits (i8_kernels.cu): scale = max |x| / 127, q = rint(x * (127 / max |x|)).
+constexpr int kQuantThreads = 256;
+template <typename T, bool VEC>
+__global__ void quantize_rows_kernel(const T* x, long long ld_x, int rows, int K, int8_t* q, long long ld_q,
+                                     float* scale);
+
+}  // namespace dels

@@ -859,21 +859,129 @@ def correction_mid_tc(
     return s_scaled
 
 
-# --------------------------------------------------------------------------- beam drafting
-@dataclass
-class BeamOut:
-    parents: torch.Tensor  # int32 [n_seq, select], the beam (0..beams-1) each child extends
-    tokens: torch.Tensor  # int64 [n_seq, select]
-    scores: torch.Tensor  # fp32 [n_seq, select], best first
+# --------------------------------------------------------------------------- 8-bit product
+_FLOATS = {torch.bfloat16: _lib.DELS_DTYPE_BF16, torch.float32: _lib.DELS_DTYPE_F32}
 
 
-_BEAM_DTYPES = {torch.bfloat16: _lib.DELS_DTYPE_BF16, torch.float32: _lib.DELS_DTYPE_F32}
+def _require_float(name: str, t: torch.Tensor, ndim: int) -> int:
+    """The DELS_DTYPE_* code of a bf16 or fp32 CUDA tensor."""
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dtype not in _FLOATS or t.dim() != ndim:
+        raise ValueError(f"{name} must be a {ndim}-D bf16 or fp32 CUDA tensor; there is no CPU path")
+    return _FLOATS[t.dtype]
 
 
 def _require_dense(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
     if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device} "
                          f"(got {t.dtype} {tuple(t.shape)} on {t.device}, stride {t.stride()})")
+
+
+def quantize_rows_i8(
+    x: torch.Tensor,
+    *,
+    q: torch.Tensor | None = None,
+    scale: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of ``x`` [rows, K] (bf16 or fp32): int8 values and fp32 [rows] scales with
+    x ~ q * scale, scale = max|row| / 127.  The rows of a ``q`` made here start on 16-byte
+    boundaries (its row stride is K rounded up to 16), as the product needs them."""
+    code = _require_float("x", x, 2)
+    dev = x.device
+    rows, K = x.shape
+    if q is None:
+        q = torch.empty(rows, -(-K // 16) * 16, dtype=torch.int8, device=dev)[:, :K]
+    elif q.dtype != torch.int8 or q.shape != (rows, K) or q.device != dev:
+        raise ValueError(f"q must be int8 {(rows, K)} on {dev} (got {q.dtype} {tuple(q.shape)} on {q.device})")
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    else:
+        _require_dense("scale", scale, torch.float32, (rows,), dev)
+    _lib.call("dels_quantize_rows_i8", _ptr(x), code, _row_major("x", x), rows, K, _ptr(q), _row_major("q", q),
+              _ptr(scale), _stream(dev))
+    return q, scale
+
+
+def _i8_operands(rows: int, K: int, dev: torch.device, wq, w_scale, bias, out, out_dtype):
+    _require_cuda("wq", wq, torch.int8, 2)
+    N = wq.shape[0]
+    if wq.shape[1] != K or wq.device != dev:
+        raise ValueError(f"wq {tuple(wq.shape)} on {wq.device} does not match inputs of width {K} on {dev}")
+    _require_dense("w_scale", w_scale, torch.float32, (N,), dev)
+    if out is None:
+        if out_dtype not in _FLOATS:
+            raise ValueError(f"out_dtype must be bf16 or fp32 (got {out_dtype})")
+        out = torch.empty(rows, N, dtype=out_dtype, device=dev)
+    else:
+        _require_float("out", out, 2)
+        if out.shape != (rows, N) or out.device != dev:
+            raise ValueError(f"out must be {(rows, N)} on {dev} (got {tuple(out.shape)} on {out.device})")
+    if bias is not None:
+        _require_dense("bias", bias, out.dtype, (N,), dev)
+    return N, out
+
+
+def linear_i8(
+    xq: torch.Tensor,
+    x_scale: torch.Tensor,
+    wq: torch.Tensor,
+    w_scale: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+    ws: Workspace | None = None,
+) -> torch.Tensor:
+    """(xq . wq^T) * x_scale[row] * w_scale[channel] (+ bias): int8 operands [rows, K] and
+    [N, K] with 16-byte aligned rows, an exact integer sum, a bf16 or fp32 result (``bias``
+    has its type)."""
+    _require_cuda("xq", xq, torch.int8, 2)
+    dev = xq.device
+    rows, K = xq.shape
+    _require_dense("x_scale", x_scale, torch.float32, (rows,), dev)
+    N, out = _i8_operands(rows, K, dev, wq, w_scale, bias, out, out_dtype)
+    ws = workspace(_lib.DELS_WS_HEADER_BYTES, dev) if ws is None else ws
+    _lib.call("dels_linear_i8", _ptr(xq), _row_major("xq", xq), _ptr(x_scale), _ptr(wq), _row_major("wq", wq),
+              _ptr(w_scale), _ptr(bias), rows, K, N, _ptr(out), _FLOATS[out.dtype], _row_major("out", out), ws.ptr,
+              ws.nbytes, _stream(dev))
+    return out
+
+
+def linear_w8a8_workspace_bytes(rows: int, K: int) -> int:
+    return int(_lib.query("dels_linear_w8a8_workspace_bytes", rows, K))
+
+
+def linear_w8a8(
+    x: torch.Tensor,
+    wq: torch.Tensor,
+    w_scale: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+    ws: Workspace | None = None,
+) -> torch.Tensor:
+    """F.linear(x, W, bias) with W = wq * w_scale[:, None] and every row of ``x`` (bf16 or
+    fp32) quantised on the way: quantize_rows_i8 and linear_i8 in one call, the weights
+    loading while the rows are quantised.  The result has x's type unless ``out`` or
+    ``out_dtype`` says otherwise."""
+    code = _require_float("x", x, 2)
+    dev = x.device
+    rows, K = x.shape
+    N, out = _i8_operands(rows, K, dev, wq, w_scale, bias, out, x.dtype if out_dtype is None else out_dtype)
+    need = linear_w8a8_workspace_bytes(rows, K)
+    ws = workspace(need, dev) if ws is None else ws.ensure(need)
+    _lib.call("dels_linear_w8a8", _ptr(x), code, _row_major("x", x), _ptr(wq), _row_major("wq", wq), _ptr(w_scale),
+              _ptr(bias), rows, K, N, _ptr(out), _FLOATS[out.dtype], _row_major("out", out), ws.ptr, ws.nbytes,
+              _stream(dev))
+    return out
+
+
+# --------------------------------------------------------------------------- beam drafting
+@dataclass
+class BeamOut:
+    parents: torch.Tensor  # int32 [n_seq, select], the beam (0..beams-1) each child extends
+    tokens: torch.Tensor  # int64 [n_seq, select]
+    scores: torch.Tensor  # fp32 [n_seq, select], best first
 
 
 def beam_select(
@@ -901,9 +1009,7 @@ def beam_select(
     only with ``pad_token`` at its score, and its logits are not read.  Masked tokens hold
     -inf or the type's lowest value; a row may be masked whole.  ``out.scores`` may be
     ``scores`` itself when ``select`` equals the beams."""
-    if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda" or logits.dim() != 2 \
-            or logits.dtype not in _BEAM_DTYPES:
-        raise ValueError("logits must be a 2-D bf16 or fp32 CUDA tensor; there is no CPU path")
+    code = _require_float("logits", logits, 2)
     dev, dtype = logits.device, logits.dtype
     rows, V = logits.shape
     if scores.dim() != 2:
@@ -935,7 +1041,7 @@ def beam_select(
     need = _lib.query("dels_beam_select_workspace_bytes", n_seq, beams, n, V)
     ws = workspace(need, dev) if ws is None else ws.ensure(need)
     _lib.call(
-        "dels_beam_select", _ptr(logits), _BEAM_DTYPES[dtype], _row_major("logits", logits), _ptr(base),
+        "dels_beam_select", _ptr(logits), code, _row_major("logits", logits), _ptr(base),
         0 if base is None else _row_major("base", base), _ptr(prior), _ptr(beta), _ptr(scores), _ptr(finished),
         int(pad_token), n_seq, beams, n, V, _ptr(out.parents), _ptr(out.tokens), _ptr(out.scores), ws.ptr, ws.nbytes,
         _stream(dev),

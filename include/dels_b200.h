@@ -340,13 +340,43 @@ DELS_API int dels_correction_mid_tc_bf16(const void* h, int64_t ld_h, const void
                                          int64_t ld_z, int B, int G, int M, const float* alpha, void* s_scaled,
                                          int64_t* keys, void* ws, size_t ws_bytes, void* stream);
 
+#define DELS_DTYPE_BF16 0
+#define DELS_DTYPE_F32 1
+
+/* ---------------------------------------------------------------------------------
+ * 8-bit integer product with a scale for each row and each channel (no counterpart in the
+ * reference): the LM head and the projections at half the bytes and twice the tensor rate
+ * of bf16.
+ *   dels_quantize_rows_i8   a = max |x[i]|, scale[i] = a / 127,
+ *                           q[i, k] = rint(x[i, k] * (127 / a)), half to even, in fp32;
+ *                           weights [N, K] once (a scale per channel), activations per call.
+ *                           A zero row gives scale 0; NaN or infinity in a row gives that
+ *                           scale and q = 0, so its products are NaN.
+ *   dels_linear_i8          out[i, n] = (sum_k xq[i, k] wq[n, k]) * x_scale[i] * w_scale[n]
+ *                           (+ bias[n]); the sum is exact, in 32-bit integers.
+ *   dels_linear_w8a8        both: quantises x into the workspace, then the product, which
+ *                           starts to load the weights while x is being quantised.
+ * x [rows, K] bf16 or fp32 with any row stride; q / xq / wq int8 with 16-byte aligned
+ * rows (ld % 16 == 0); out and bias bf16 or fp32 (out_dtype), any row stride.
+ * K <= DELS_I8_MAX_K.  ws: DELS_WS_HEADER_BYTES for dels_linear_i8,
+ * dels_linear_w8a8_workspace_bytes(rows, K) for dels_linear_w8a8.
+ * --------------------------------------------------------------------------------- */
+#define DELS_I8_MAX_K 131071 /* 2^31 / 128^2 - 1 */
+DELS_API int dels_quantize_rows_i8(const void* x, int dtype, int64_t ld_x, int rows, int K, int8_t* q, int64_t ld_q,
+                                   float* scale, void* stream);
+DELS_API int dels_linear_i8(const int8_t* xq, int64_t ld_xq, const float* x_scale, const int8_t* wq, int64_t ld_wq,
+                            const float* w_scale, const void* bias, int rows, int K, int N, void* out, int out_dtype,
+                            int64_t ld_out, void* ws, size_t ws_bytes, void* stream);
+DELS_API size_t dels_linear_w8a8_workspace_bytes(int rows, int K);
+DELS_API int dels_linear_w8a8(const void* x, int x_dtype, int64_t ld_x, const int8_t* wq, int64_t ld_wq,
+                              const float* w_scale, const void* bias, int rows, int K, int N, void* out, int out_dtype,
+                              int64_t ld_out, void* ws, size_t ws_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------------
  * Beam drafting (no counterpart in the reference, which drafts one chain per sequence):
  * a sequence keeps `beams` candidate chains, each step extends every chain by every
  * token, and the best `select` of these candidates go on.
  * --------------------------------------------------------------------------------- */
-#define DELS_DTYPE_BF16 0
-#define DELS_DTYPE_F32 1
 #define DELS_BEAM_MAX 64          /* beams and select are at most this */
 #define DELS_BEAM_MAX_VOCAB 524288
 
