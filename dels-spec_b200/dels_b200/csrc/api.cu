@@ -28,6 +28,8 @@ constexpr int kVersion = 1;
 constexpr int kMaxDevices = 64;
 // Split-K sizing of the projection GEMMs aims at this many CTAs (one B200 wave).
 constexpr int kTargetCtas = 148;
+// Most SMs that workspace sizes are computed for.
+constexpr int kMaxSmCount = 160;
 // Scorer schedule: 16 row tiles (2048 rows, a 17.8 MB A panel at H + r = 4352) sweep
 // the vocabulary together; the last partial wave's tiles are split 4 ways along N.
 constexpr int kScorerGroupM = 16;
@@ -214,8 +216,7 @@ cudaError_t set_smem(K kernel, int bytes) {
 }
 
 constexpr int kMaxSmem = 232448;
-constexpr int kBeamRowSmemMax = kBeamMax * kBeamGroup * (int)sizeof(uint32_t);
-static_assert(kBeamMaxGroups * (int)sizeof(uint32_t) <= kBeamRowSmemMax, "group keys fit");
+constexpr int kBeamFinishSmemMax = beam_finish_smem(kBeamMax, kBeamMax, kBeamFinishWarps, kBeamMax * 32 * 4);
 
 int init_device(int dev) {
   if (dev < 0 || dev >= kMaxDevices) return fail(DELS_ERR_INVALID_ARG, "device %d out of range", dev);
@@ -237,6 +238,13 @@ int init_device(int dev) {
   if (major != 10 || minor != 0) {
     rc = fail(DELS_ERR_UNSUPPORTED, "device %d is sm_%d%d; this library is built for sm_100a only", dev, major, minor);
   } else {
+// as SET, for kernels whose residency is planned by an SM's whole shared memory, and for those
+// that run between them (a change of the split takes time)
+#define SET_SHARED(k, b)                                                                                       \
+  SET(k, b)                                                                                                    \
+  if (rc == DELS_OK && (e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout,            \
+                                                 cudaSharedmemCarveoutMaxShared)) != cudaSuccess)              \
+    rc = cuda_fail(e, "kernel setup: " #k);
 #define SET(k, b)                                            \
   if (rc == DELS_OK && (e = set_smem(k, b)) != cudaSuccess) rc = cuda_fail(e, "kernel setup: " #k);
     SET((tc_gemm_kernel<256, kArgmax, false>), TcConfig<256>::kSmemBytes);
@@ -279,19 +287,22 @@ int init_device(int dev) {
     SET(gru_gates_kernel, 0);
     SET(gru_finalize_kernel, 0);
     SET(wait_selftest_kernel, 0);
-    SET((beam_scan_kernel<float, false, false>), 0);
-    SET((beam_scan_kernel<float, false, true>), 0);
-    SET((beam_scan_kernel<float, true, false>), 0);
-    SET((beam_scan_kernel<float, true, true>), 0);
-    SET((beam_scan_kernel<__nv_bfloat16, false, false>), 0);
-    SET((beam_scan_kernel<__nv_bfloat16, false, true>), 0);
-    SET((beam_scan_kernel<__nv_bfloat16, true, false>), 0);
-    SET((beam_scan_kernel<__nv_bfloat16, true, true>), 0);
-    SET((beam_row_kernel<float, false>), kBeamRowSmemMax);
-    SET((beam_row_kernel<float, true>), kBeamRowSmemMax);
-    SET((beam_row_kernel<__nv_bfloat16, false>), kBeamRowSmemMax);
-    SET((beam_row_kernel<__nv_bfloat16, true>), kBeamRowSmemMax);
-    SET(beam_merge_kernel, kBeamMax * kBeamMax * (int)sizeof(uint32_t));
+    SET_SHARED((beam_scan_kernel<float, false, false>), 0);
+    SET_SHARED((beam_scan_kernel<float, false, true>), kBeamScanSmemMax);
+    SET_SHARED((beam_scan_kernel<float, true, false>), 0);
+    SET_SHARED((beam_scan_kernel<float, true, true>), kBeamScanSmemMax);
+    SET_SHARED((beam_scan_kernel<__nv_bfloat16, false, false>), 0);
+    SET_SHARED((beam_scan_kernel<__nv_bfloat16, false, true>), kBeamScanSmemMax);
+    SET_SHARED((beam_scan_kernel<__nv_bfloat16, true, false>), 0);
+    SET_SHARED((beam_scan_kernel<__nv_bfloat16, true, true>), kBeamScanSmemMax);
+    SET_SHARED((beam_finish_kernel<float, false, false>), kBeamFinishSmemMax);
+    SET_SHARED((beam_finish_kernel<float, false, true>), kBeamFinishSmemMax);
+    SET_SHARED((beam_finish_kernel<float, true, false>), kBeamFinishSmemMax);
+    SET_SHARED((beam_finish_kernel<float, true, true>), kBeamFinishSmemMax);
+    SET_SHARED((beam_finish_kernel<__nv_bfloat16, false, false>), kBeamFinishSmemMax);
+    SET_SHARED((beam_finish_kernel<__nv_bfloat16, false, true>), kBeamFinishSmemMax);
+    SET_SHARED((beam_finish_kernel<__nv_bfloat16, true, false>), kBeamFinishSmemMax);
+    SET_SHARED((beam_finish_kernel<__nv_bfloat16, true, true>), kBeamFinishSmemMax);
     SET(beam_reorder_kernel, 0);
     SET((i8_gemm_kernel<16, __nv_bfloat16>), I8Config<16>::kSmemBytes);
     SET((i8_gemm_kernel<32, __nv_bfloat16>), I8Config<32>::kSmemBytes);
@@ -308,6 +319,7 @@ int init_device(int dev) {
     SET((quantize_rows_kernel<__nv_bfloat16, false>), 0);
     SET((quantize_rows_kernel<__nv_bfloat16, true>), 0);
 #undef SET
+#undef SET_SHARED
   }
   if (rc == DELS_OK) {
     // A persistent grid of CTA pairs must fit on the device at once: ask the occupancy
@@ -720,48 +732,57 @@ int fused_argmax_common(const void* h, long long ld_h, const void* W, long long 
   return launch_tc<256, kArgmax, false>(op, a, ds->sm_count, st);
 }
 
-// Lays out the scratch of a selection over `base` (counted only when `a` is null); returns
-// its bytes.
-size_t beam_scratch(int n_seq, int beams, int select, int V, char* base, BeamSelectArgs* a) {
+// Plans a selection's scan and lays out its scratch over `base` (counted only when `a` is
+// null); returns the scratch's bytes.
+size_t beam_plan(int n_seq, int beams, int V, int elem, bool mix, int sm_count, char* base, BeamSelectArgs* a) {
   const size_t rows = (size_t)n_seq * beams;
   const int groups = cdiv(V, kBeamGroup);
-  // enough CTAs to fill the device several times over, and at least one group for each warp
-  const int per_cta = kBeamThreads / 32;
-  const long long want = rows < 8ll * kTargetCtas ? cdiv(8ll * kTargetCtas, (long long)rows) : 1;
-  const int most = cdiv(groups, per_cta);
-  const int slices = want < most ? (int)want : most;
-  size_t at = 0;
-  const size_t key0 = at;
-  at += align256(rows * groups * sizeof(uint32_t));
-  const size_t part0 = at;
-  at += align256(rows * slices * sizeof(float2));
-  const size_t best0 = at;
-  at += align256(rows * select * sizeof(BeamEntry));
-  const size_t stat0 = at;
-  at += align256(rows * sizeof(float2));
+  const int scan_rows = mix ? (beams < kBeamScanRows ? beams : kBeamScanRows) : 1;
+  const int blocks = n_seq * cdiv(beams, scan_rows);
+  // As many CTAs as the device holds at once, by the shared memory of an SM and the kernel's
+  // registers, with a group for each of their teams at least.
+  const int smem = beam_scan_smem(scan_rows, elem, mix) + 2048;
+  const int fit = (220 << 10) / smem, most = mix ? 5 : 8;
+  const long long units = (long long)blocks * groups;
+  const long long teams = scan_teams(scan_rows);
+  long long ctas = (long long)(fit < most ? fit : most) * sm_count;
+  if (ctas > (units + teams - 1) / teams) ctas = (units + teams - 1) / teams;
+  // CTAs that can share a block: those of floor(units / ctas) groups or more, and one cut off
+  // at either end
+  const int parts = (int)(groups / (units / ctas)) + 2;
+  const size_t part0 = align256(rows * groups * sizeof(float4));
   if (a != nullptr) {
     a->groups = groups;
-    a->slices = slices;
-    a->ws.group_key = reinterpret_cast<uint32_t*>(base + key0);
+    a->parts = parts;
+    a->scan_rows = scan_rows;
+    a->scan_ctas = (int)ctas;
+    a->share.per = (int)(units / ctas);
+    a->share.more = (int)(units % ctas);
+    a->ws.group_top = reinterpret_cast<float4*>(base);
     a->ws.part = reinterpret_cast<float2*>(base + part0);
-    a->ws.best = reinterpret_cast<BeamEntry*>(base + best0);
-    a->ws.stat = reinterpret_cast<float2*>(base + stat0);
   }
-  return at;
+  return part0 + align256(rows * parts * sizeof(float2));
 }
 
 template <typename T, bool MIX>
-int launch_beam_select(const BeamSelectArgs& a, bool vec, cudaStream_t st) {
-  const int rows = a.n_seq * a.beams;
+int launch_beam_select(BeamSelectArgs a, bool vec, cudaStream_t st) {
+  a.slot_bytes = beam_slot_bytes(a.scan_rows, sizeof(T), MIX);
   DELS_CHECK_PDL("beam_scan_kernel launch",
                  launch_pdl(vec ? beam_scan_kernel<T, MIX, true> : beam_scan_kernel<T, MIX, false>,
-                            dim3((unsigned)(rows * a.slices)), dim3(kBeamThreads), 0, st, a));
-  const int group_keys = a.select * kBeamGroup > a.groups ? a.select * kBeamGroup : a.groups;
-  DELS_CHECK_PDL("beam_row_kernel launch", launch_pdl(beam_row_kernel<T, MIX>, dim3((unsigned)rows),
-                                                      dim3(kBeamThreads), group_keys * sizeof(uint32_t), st, a));
-  DELS_CHECK_PDL("beam_merge_kernel launch",
-                 launch_pdl(beam_merge_kernel, dim3((unsigned)a.n_seq), dim3(kBeamThreads),
-                            (size_t)a.beams * a.select * sizeof(uint32_t), st, a));
+                            dim3((unsigned)a.scan_ctas), dim3(32 * scan_pairs(a.scan_rows) * scan_teams(a.scan_rows)),
+                            vec ? beam_scan_smem(a.scan_rows, sizeof(T), MIX) : 0, st, a));
+  // Sixteen warps or nearly: several share a beam's groups where there are few beams.  The bound
+  // needs some more maxima than candidates: a lane offers its four quarters' where its
+  // largest alone would be too few.
+  const int split = a.beams >= kBeamFinishWarps ? 1 : kBeamFinishWarps / a.beams;
+  const int lanes = a.groups < 32 * split ? a.groups : 32 * split;
+  a.finish_split = split;
+  a.finish_values = a.beams * lanes < 4 * a.select ? 4 : 1;
+  const int warps = split * (a.beams < kBeamFinishWarps ? a.beams : kBeamFinishWarps);
+  DELS_CHECK_PDL("beam_finish_kernel launch",
+                 launch_pdl(vec ? beam_finish_kernel<T, MIX, true> : beam_finish_kernel<T, MIX, false>,
+                            dim3((unsigned)a.n_seq), dim3(32 * warps),
+                            beam_finish_smem(a.beams, a.select, warps, a.beams * split * 32 * a.finish_values), st, a));
   return DELS_OK;
 }
 
@@ -1566,7 +1587,13 @@ int dels_gather_scaled_rows_bf16(const int64_t* tokens, int64_t tok_stride, int 
 
 size_t dels_beam_select_workspace_bytes(int n_seq, int beams, int select, int V) {
   if (n_seq <= 0 || beams <= 0 || select <= 0 || V <= 0) return DELS_WS_HEADER_BYTES;
-  return DELS_WS_HEADER_BYTES + beam_scratch(n_seq, beams, select, V, nullptr, nullptr);
+  // whatever the device, the type and whether logits are shared
+  size_t most = 0;
+  for (int i = 0; i < 4; ++i) {
+    const size_t n = beam_plan(n_seq, beams, V, i & 1 ? 4 : 2, (i & 2) != 0, kMaxSmCount, nullptr, nullptr);
+    most = n > most ? n : most;
+  }
+  return DELS_WS_HEADER_BYTES + most;
 }
 
 int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const void* base, int64_t ld_base,
@@ -1579,8 +1606,8 @@ int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const voi
     return fail(DELS_ERR_INVALID_ARG, "beams and select must be in 1..%d (got %d, %d)", kBeamMax, beams, select);
   if (V < select || V > DELS_BEAM_MAX_VOCAB)
     return fail(DELS_ERR_INVALID_ARG, "V must be in select..%d (got %d, select %d)", DELS_BEAM_MAX_VOCAB, V, select);
-  if ((long long)n_seq * beams > (1ll << 22))
-    return fail(DELS_ERR_INVALID_ARG, "at most 2^22 rows (got %lld)", (long long)n_seq * beams);
+  if ((long long)n_seq * beams > (1ll << 20))  // groups of all rows are counted in 32 bits
+    return fail(DELS_ERR_INVALID_ARG, "at most 2^20 rows (got %lld)", (long long)n_seq * beams);
   if (dtype != DELS_DTYPE_BF16 && dtype != DELS_DTYPE_F32) return fail(DELS_ERR_INVALID_ARG, "unknown dtype %d", dtype);
   const size_t elem = dtype == DELS_DTYPE_BF16 ? 2 : 4;
   if (n_seq > 0 && (logits == nullptr || cum == nullptr || parents == nullptr || tokens == nullptr || scores == nullptr))
@@ -1616,11 +1643,14 @@ int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const voi
   a.parents = parents;
   a.tokens = reinterpret_cast<long long*>(tokens);
   a.scores = scores;
-  beam_scratch(n_seq, beams, select, V, static_cast<char*>(ws) + DELS_WS_HEADER_BYTES, &a);
-  // 16-byte loads need every row to start on a 16-byte boundary
-  const bool vec = aligned16(logits) && (ld_logits * elem) % 16 == 0 &&
+  a.status = hdr.status;
+  // 16-byte loads of eight logits need every row to start on a 16-byte boundary and to end
+  // with a whole load
+  const bool vec = V % 8 == 0 && aligned16(logits) && (ld_logits * elem) % 16 == 0 &&
                    (base == nullptr || (aligned16(base) && (ld_base * elem) % 16 == 0)) && aligned16(prior);
   const bool mix = base != nullptr || prior != nullptr;
+  beam_plan(n_seq, beams, V, (int)elem, mix, ds->sm_count < kMaxSmCount ? ds->sm_count : kMaxSmCount,
+            static_cast<char*>(ws) + DELS_WS_HEADER_BYTES, &a);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == DELS_DTYPE_BF16 ? (mix ? launch_beam_select<__nv_bfloat16, true>(a, vec, st)
                                          : launch_beam_select<__nv_bfloat16, false>(a, vec, st))

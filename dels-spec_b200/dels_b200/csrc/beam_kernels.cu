@@ -10,17 +10,24 @@
 // (masks) cancel before they meet anything small.  The best `select` candidates of a
 // sequence: higher score, then lower beam, then larger x, then lower token.
 //
-//   beam_scan_kernel   one pass over the logits: per slice of a row the running (m, S) of
-//                      an online softmax, and the maximum of every group of logits.
-//   beam_row_kernel    the row's `select` best groups by (maximum, lowest group) hold its
-//                      `select` best logits: a logit outside them is beaten by one in each.
-//                      They are read again and their best logits kept, in order.
-//   beam_merge_kernel  scores of all beams' lists, the best `select` of them.
+//   beam_scan_kernel    one pass over the logits: per slice of a row the running (m, S) of
+//                       an online softmax, and for every 512 logits the maxima of their four
+//                       quarters.
+//   beam_finish_kernel  a CTA per sequence, a warp per beam.  The `select`-th largest of 128
+//                       of those maxima bounds the row's `select` best logits from below, so
+//                       only the quarters that reach it are read again; then the beams' lists
+//                       meet in shared memory.
+//
+// Both kernels are short loops on purpose: a step of one sequence runs each instruction a
+// few times only, and then fetching code costs more than executing it (unrolled over four
+// rows, the scan of 4 x 151936 logits took 23 us for 810 instructions a warp).
 #include "beam_kernels.cuh"
 
 namespace dels {
 
 namespace {
+
+constexpr uint32_t kAllLanes = 0xffffffffu;
 
 __device__ __forceinline__ float neg_inf() { return -__int_as_float(0x7f800000); }
 
@@ -38,10 +45,27 @@ __device__ __forceinline__ float warp_max_nan(float v) {
   return r;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// 2^x by the special-function unit (relative error of 2^-22).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two packed fp32 additions or products in one instruction, each rounded by itself.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
 }
 
 // (m, s) of two parts of a softmax; s counts exp(x - m).
@@ -53,266 +77,859 @@ __device__ __forceinline__ float2 softmax_join(float2 a, float2 b) {
   return make_float2(m, a.y * ea + b.y * eb);
 }
 
-// x[v] of one logit.  Every operation is rounded by itself, in this order.
+// ------------------------------------------------------------------ logits
+// A lane's kPer logits of a group.  VEC (16-byte loads: rows aligned to 16 bytes, V a
+// multiple of 8): two runs of eight, run h of lane l at 256 h + 8 l.  Otherwise every 32nd.
+constexpr int kPer = kBeamGroup / 32;
+
+// Quarter q of a group is the lanes' logits 4 q .. 4 q + 3; their offsets in the group.
+template <bool VEC>
+__device__ __forceinline__ int quarter_offset(int q, int lane, int j) {
+  return VEC ? (q >> 1) * 256 + lane * 8 + (q & 1) * 4 + j : (4 * q + j) * 32 + lane;
+}
+
+// Four logits of a lane as they are loaded.
+template <typename T>
+struct Raw4;
+template <>
+struct Raw4<float> {
+  float4 w;
+  __device__ __forceinline__ void load(const float* p) {
+    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w)
+                 : "l"(p));
+  }
+  __device__ __forceinline__ void unpack(float2 (&x)[2]) const { x[0] = make_float2(w.x, w.y), x[1] = make_float2(w.z, w.w); }
+};
+template <>
+struct Raw4<__nv_bfloat16> {
+  uint2 w;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "l"(p));
+  }
+  __device__ __forceinline__ void unpack(float2 (&x)[2]) const {
+    x[0] = make_float2(bf16_lo(w.x), bf16_hi(w.x)), x[1] = make_float2(bf16_lo(w.y), bf16_hi(w.y));
+  }
+};
+
+// A lane's logits of a group from their staged copy.
+__device__ __forceinline__ void staged(const float* group, int lane, float2 (&x)[kPer / 2]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 w = *reinterpret_cast<const float4*>(group + (i >> 1) * 256 + lane * 8 + (i & 1) * 4);
+    x[2 * i] = make_float2(w.x, w.y), x[2 * i + 1] = make_float2(w.z, w.w);
+  }
+}
+__device__ __forceinline__ void staged(const __nv_bfloat16* group, int lane, float2 (&x)[kPer / 2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint4 w = *reinterpret_cast<const uint4*>(group + h * 256 + lane * 8);
+    x[4 * h] = make_float2(bf16_lo(w.x), bf16_hi(w.x)), x[4 * h + 1] = make_float2(bf16_lo(w.y), bf16_hi(w.y));
+    x[4 * h + 2] = make_float2(bf16_lo(w.z), bf16_hi(w.z)), x[4 * h + 3] = make_float2(bf16_lo(w.w), bf16_hi(w.w));
+  }
+}
+
+// Starts the copy of `bytes` (a multiple of 16) to shared memory, counted on `bar`.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// The draft logits and prior that a sequence's beams share; either may be missing.
+template <typename T>
+struct Shared {
+  const T* base;
+  const float* prior;
+  float nbeta;  // -beta
+};
+
+// x = (base + logit) - beta prior, every operation rounded by itself.
 template <typename T, bool MIX>
-__device__ __forceinline__ float mixed_logit(const T* row, const T* base, const float* prior, float beta, int v) {
+__device__ __forceinline__ float mixed_logit(const T* row, const Shared<T>& sh, int v) {
   float x = to_f32(row[v]);
   if constexpr (MIX) {
-    if (base != nullptr) x = __fadd_rn(to_f32(base[v]), x);
-    if (prior != nullptr) x = __fsub_rn(x, __fmul_rn(beta, __ldg(prior + v)));
+    if (sh.base != nullptr) x = __fadd_rn(to_f32(sh.base[v]), x);
+    if (sh.prior != nullptr) x = __fadd_rn(x, __fmul_rn(sh.nbeta, __ldg(sh.prior + v)));
   }
   return x;
 }
 
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = __ldcs(reinterpret_cast<const float4*>(p));
-  const float4 b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 w = __ldcs(reinterpret_cast<const uint4*>(p));
-  x[0] = bf16_lo(w.x), x[1] = bf16_hi(w.x), x[2] = bf16_lo(w.y), x[3] = bf16_hi(w.y);
-  x[4] = bf16_lo(w.z), x[5] = bf16_hi(w.z), x[6] = bf16_lo(w.w), x[7] = bf16_hi(w.w);
+// A lane's logits of the group at v0 without 16-byte loads; -inf past V.
+template <typename T, bool MIX>
+__device__ __forceinline__ void load_single(const T* row, const Shared<T>& sh, int v0, int V, int lane,
+                                            float2 (&x)[kPer / 2]) {
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i) {
+    const int u = v0 + 64 * i + lane, v = u + 32;
+    x[i].x = u < V ? mixed_logit<T, MIX>(row, sh, u) : neg_inf();
+    x[i].y = v < V ? mixed_logit<T, MIX>(row, sh, v) : neg_inf();
+  }
 }
 
-// Positions of the n largest of keys[0..N) in shared memory (equal keys: lowest positions),
-// ascending, into pos[0..n).  All threads of the block call it; n <= N, n <= kBeamMax.
-// The n-th largest key comes from a bisection over the keys' common leading bits; then one
-// warp walks the keys in order.
-__device__ void block_top_positions(const uint32_t* keys, int N, int n, int* pos, uint32_t* shared4) {
-  const int t = threadIdx.x;
-  if (N <= n) {
-    for (int i = t; i < N; i += kBeamThreads) pos[i] = i;
-    __syncthreads();
-    return;
+// Takes a lane's logits of a group of N rows into their running softmax (m, the same in all
+// lanes, and the lane's own sums s); t: the maxima of the quarters, NaN where one holds it,
+// and then the sums are NaN.  Two rows at a time fill each other's waits.
+template <int N>
+__device__ __forceinline__ void fold_group(const float2 (&x)[N][kPer / 2], float (&m)[N], float2 (&s)[N],
+                                           float4 (&t)[N]) {
+  float nref[N];
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    float q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      q[i] = fmax_nan(fmax3_nan(x[r][2 * i].x, x[r][2 * i].y, x[r][2 * i + 1].x), x[r][2 * i + 1].y);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = warp_max_nan(q[i]);
+    t[r] = make_float4(q[0], q[1], q[2], q[3]);
   }
-  // shared4[0]: count of the bisection step, [1] / [2]: smallest and largest key
-  if (t == 0) shared4[0] = 0, shared4[1] = 0xFFFFFFFFu, shared4[2] = 0;
-  __syncthreads();
-  uint32_t lo = 0xFFFFFFFFu, hi = 0;
-  for (int i = t; i < N; i += kBeamThreads) {
-    lo = min(lo, keys[i]);
-    hi = max(hi, keys[i]);
-  }
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  if ((t & 31) == 0) {
-    atomicMin(&shared4[1], lo);
-    atomicMax(&shared4[2], hi);
-  }
-  __syncthreads();
-  lo = shared4[1];
-  hi = shared4[2];
-  // largest T with count(keys >= T) >= n, in [lo, hi]
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2 + 1;
-    int c = 0;
-    for (int i = t; i < N; i += kBeamThreads) c += keys[i] >= mid;
-    c = __reduce_add_sync(0xffffffffu, c);
-    if ((t & 31) == 0) atomicAdd(&shared4[0], (uint32_t)c);
-    __syncthreads();
-    const uint32_t total = shared4[0];
-    __syncthreads();
-    if (t == 0) shared4[0] = 0;
-    __syncthreads();
-    if (total >= (uint32_t)n) {
-      lo = mid;
-      if (total == (uint32_t)n) break;
-    } else {
-      hi = mid - 1;
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    const float top = fmax3_nan(fmax_nan(t[r].x, t[r].y), t[r].z, t[r].w);
+    if (top > m[r]) {
+      const float down = __expf(m[r] - top);  // m = -inf: the sums are 0 and stay 0
+      s[r] = mul2(s[r], make_float2(down, down));
+      m[r] = top;
     }
+    nref[r] = m[r] == neg_inf() ? 0.0f : -m[r];
   }
-  if (t < 32) {
-    int above = 0;
-    for (int i = t; i < N; i += 32) above += keys[i] > lo;
-    above = __reduce_add_sync(0xffffffffu, above);
-    // above < n unless the bisection stopped early on an exact count, when it is <= n
-    int ties = n - above, at = 0;
-    for (int i0 = 0; i0 < N && at < n; i0 += 32) {
-      const int i = i0 + t;
-      const uint32_t k = i < N ? keys[i] : 0u;
-      const uint32_t same = __ballot_sync(0xffffffffu, i < N && k == lo);
-      const bool tie = i < N && k == lo && __popc(same & ((1u << t) - 1u)) < ties;
-      const uint32_t take = __ballot_sync(0xffffffffu, (i < N && k > lo) || tie);
-      if ((take >> t) & 1u) pos[at + __popc(take & ((1u << t) - 1u))] = i;
-      at += __popc(take);
-      ties -= min(ties, __popc(same));
+#pragma unroll
+  for (int i = 0; i < kPer / 2; ++i)
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      const float2 e =
+          mul2(add2(x[r][i], make_float2(nref[r], nref[r])), make_float2(1.4426950408889634f, 1.4426950408889634f));
+      s[r] = add2(s[r], make_float2(exp2_approx(e.x), exp2_approx(e.y)));
     }
-  }
-  __syncthreads();
 }
 
 }  // namespace
 
+// ------------------------------------------------------------------ the scan
+// A block of rows is one row, or (MIX) up to kBeamScanRows beams of a sequence, which meet
+// the draft logits and prior they share in one CTA.  A team of warps scans a group, two rows
+// a warp; the teams of a CTA take turns at the groups of its run: of one block, or of the end
+// of one and the start of the next.  Each row's (m, S) of a CTA's share goes to part[row][CTA
+// - first CTA of the block].  With VEC a team has the next groups copied into its ring in
+// shared memory ahead of its arithmetic (bulk copies: no registers held, a handful of
+// instructions a group).
 template <typename T, bool MIX, bool VEC>
-__global__ void __launch_bounds__(kBeamThreads) beam_scan_kernel(const BeamSelectArgs a) {
-  __shared__ float2 warp_part[kBeamThreads / 32];
-  const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
+__global__ void __launch_bounds__(32 * kBeamScanWarps, MIX ? 5 : 8) beam_scan_kernel(const BeamSelectArgs a) {
+  constexpr int D = beam_scan_depth(sizeof(T), MIX);
+  constexpr int N = MIX ? 2 : 1;  // rows of a warp
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float2 team_part[kBeamScanWarps][kBeamScanRows];
+  __shared__ uint64_t full[kBeamScanWarps][D], empty[kBeamScanWarps][D];  // [team][slot]
+  __shared__ int aborted;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
-  if (a.finished != nullptr && a.finished[row] != 0) return;
-  const T* logits = static_cast<const T*>(a.logits) + (long long)row * a.ld;
-  const T* base = nullptr;
-  float beta = 0.0f;
-  if constexpr (MIX) {
-    if (a.base != nullptr) base = static_cast<const T*>(a.base) + (long long)(row / a.beams) * a.ld_base;
-    if (a.prior != nullptr) beta = __ldg(a.beta);
+  const int pairs = scan_pairs(a.scan_rows), teams = (blockDim.x >> 5) / pairs;
+  const int team = warp / pairs, pair = warp % pairs;
+  const int blocks_per_seq = (a.beams + a.scan_rows - 1) / a.scan_rows;
+  int unit = a.share.first(blockIdx.x);
+  const int unit_end = a.share.first(blockIdx.x + 1);
+  char* ring = smem + team * D * a.slot_bytes;
+  if (threadIdx.x == 0) {
+    aborted = 0;
+    for (int i = 0; i < kBeamScanWarps * D; ++i) {
+      mbar_init(smem_u32(&full[0][0] + i), 1);
+      mbar_init(smem_u32(&empty[0][0] + i), pairs);
+    }
+    mbar_fence_init();
   }
-  const int per_slice = (a.groups + a.slices - 1) / a.slices;
-  const int g_end = min(a.groups, (slice + 1) * per_slice);
-  float m = neg_inf(), s = 0.0f;  // m is the same in all lanes, s the lane's own sum
-  for (int g = slice * per_slice + warp; g < g_end; g += kBeamThreads / 32) {
-    const int v0 = g * kBeamGroup;
-    float x[8];
-    if (VEC && v0 + kBeamGroup <= a.V) {
-      const int v = v0 + lane * 8;
-      load8(logits + v, x);
-      if constexpr (MIX) {
-        if (base != nullptr) {
-          float b[8];
-          load8(base + v, b);
+  __syncthreads();
+  pdl_wait();
+  int slot = 0, fill_slot = 0;
+  uint32_t parity = 0, fill_parity = 0;
+#pragma unroll 1
+  while (unit < unit_end) {
+    const int block = unit / a.groups, g_begin = unit - block * a.groups;
+    const int g_end = min(a.groups, g_begin + (unit_end - unit));
+    unit += g_end - g_begin;
+    const int seq = block / blocks_per_seq;
+    const int row0 = seq * a.beams + block % blocks_per_seq * a.scan_rows;
+    const int n_rows = min(a.scan_rows, (seq + 1) * a.beams - row0);
+    const T* logits = static_cast<const T*>(a.logits) + (long long)row0 * a.ld;
+    // the rows to scan: lane i < n_live holds the i-th one
+    const bool mine = lane < n_rows && (a.finished == nullptr || a.finished[row0 + lane] == 0);
+    const uint32_t live = __ballot_sync(kAllLanes, mine);
+    const int n_live = __popc(live);
+    if (n_live == 0) continue;
+    int my_row = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = __fadd_rn(b[j], x[j]);
-        }
-        if (a.prior != nullptr) {
-          const float4 p = __ldg(reinterpret_cast<const float4*>(a.prior + v));
-          const float4 q = __ldg(reinterpret_cast<const float4*>(a.prior + v) + 1);
-          const float pr[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+    for (int r = 0; r < kBeamScanRows; ++r)
+      if (((live >> r) & 1u) && __popc(live & ((1u << r) - 1u)) == lane) my_row = r;
+    const int n_mine = min(N, n_live - N * pair);  // rows of this warp, from the N pair-th on
+    Shared<T> sh{nullptr, nullptr, 0.0f};
+    if constexpr (MIX) {
+      if (a.base != nullptr) sh.base = static_cast<const T*>(a.base) + (long long)seq * a.ld_base;
+      if (a.prior != nullptr) sh.prior = a.prior, sh.nbeta = -__ldg(a.beta);
+    }
+    float m[N];
+    float2 s[N];
+    float4* tops[N];
+    const T* row[N];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = __fsub_rn(x[j], __fmul_rn(beta, pr[j]));
-        }
+    for (int r = 0; r < N; ++r) {
+      m[r] = neg_inf();
+      s[r] = make_float2(0.0f, 0.0f);
+      const int k = __shfl_sync(kAllLanes, my_row, min(N * pair + r, n_live - 1));
+      tops[r] = a.ws.group_top + (long long)(row0 + k) * a.groups;
+      row[r] = logits + k * a.ld;
+    }
+    // Lane i < n_live of the team's first warp copies the i-th row's part of a group into a
+    // slot, the next two lanes those of the draft logits and the prior.
+    const char* src = nullptr;
+    uint32_t src_elem = sizeof(T);
+    if (lane < n_live) src = reinterpret_cast<const char*>(logits + my_row * a.ld);
+    if constexpr (MIX) {
+      if (lane == n_live && sh.base != nullptr) src = reinterpret_cast<const char*>(sh.base);
+      if (lane == n_live + 1 && sh.prior != nullptr) src = reinterpret_cast<const char*>(sh.prior), src_elem = 4;
+    }
+    const uint32_t token_bytes = __reduce_add_sync(kAllLanes, src != nullptr ? src_elem : 0u);
+    const uint32_t dst = smem_u32(ring) + lane * kBeamGroup * sizeof(T);
+    auto copy = [&](int k) {
+      if (pair != 0 || k >= g_end) return;
+      // a wait that gives up leaves its mark in the status word; the CTA then runs through
+      mbar_wait(smem_u32(&empty[team][fill_slot]), fill_parity ^ 1u, &aborted, a.status);
+      const uint32_t len = min(kBeamGroup, a.V - k * kBeamGroup), bar = smem_u32(&full[team][fill_slot]);
+      if (lane == 0) mbar_arrive_expect_tx(bar, len * token_bytes);
+      __syncwarp();
+      if (src != nullptr)
+        bulk_copy(dst + fill_slot * a.slot_bytes, src + (long long)k * kBeamGroup * src_elem, len * src_elem, bar);
+      if (++fill_slot == D) fill_slot = 0, fill_parity ^= 1u;
+    };
+    int g = g_begin + team;
+    if (VEC) {
+#pragma unroll 1
+      for (int i = 0; i < D - 1; ++i) copy(g + i * teams);
+    }
+#pragma unroll 1
+    for (; g < g_end; g += teams) {
+      const T* p = reinterpret_cast<const T*>(ring + slot * a.slot_bytes);
+      const uint32_t read = smem_u32(&empty[team][slot]);
+      if constexpr (VEC) {
+        copy(g + (D - 1) * teams);
+        mbar_wait(smem_u32(&full[team][slot]), parity, &aborted, a.status);
+        if (++slot == D) slot = 0, parity ^= 1u;
       }
+      if (n_mine <= 0) {
+        if (VEC && lane == 0) mbar_arrive(read);
+        continue;
+      }
+      const int past = a.V - g * kBeamGroup - lane * 8;  // logits from here on, for the lane
+      const bool short_group = a.V - g * kBeamGroup < kBeamGroup;
+      float2 x[N][kPer / 2];
+      if constexpr (VEC) {
+#pragma unroll
+        for (int r = 0; r < N; ++r) staged(p + (N * pair + (r < n_mine ? r : 0)) * kBeamGroup, lane, x[r]);
+        if constexpr (MIX) {
+          float2 y[kPer / 2];
+          if (sh.base != nullptr) {
+            staged(p + n_live * kBeamGroup, lane, y);
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i)
+#pragma unroll
+              for (int r = 0; r < N; ++r) x[r][i] = add2(y[i], x[r][i]);
+          }
+          if (sh.prior != nullptr) {
+            staged(reinterpret_cast<const float*>(p + (n_live + 1) * kBeamGroup), lane, y);
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) {
+              y[i] = mul2(make_float2(sh.nbeta, sh.nbeta), y[i]);
+#pragma unroll
+              for (int r = 0; r < N; ++r) x[r][i] = add2(x[r][i], y[i]);
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(read);
+        if (short_group) {
+#pragma unroll
+          for (int i = 0; i < kPer / 2; ++i)
+            if (past <= (i >> 2) * 256) {
+#pragma unroll
+              for (int r = 0; r < N; ++r) x[r][i] = make_float2(neg_inf(), neg_inf());
+            }
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < N; ++r) load_single<T, MIX>(row[r], sh, g * kBeamGroup, a.V, lane, x[r]);
+      }
+      float4 t[N];
+      fold_group<N>(x, m, s, t);
+#pragma unroll
+      for (int r = 0; r < N; ++r)
+        if (lane == r && r < n_mine) tops[r][g] = t[r];
+    }
+    __syncthreads();  // the block before has been joined, and all slots are read
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      float sum = s[r].x + s[r].y;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, o);
+      if (lane == 0 && r < n_mine) team_part[team][N * pair + r] = make_float2(m[r], sum);
+    }
+    __syncthreads();
+    if (warp == 0 && lane < n_live) {
+      float2 p = team_part[0][lane];
+#pragma unroll 1
+      for (int w = 1; w < teams; ++w) p = softmax_join(p, team_part[w][lane]);
+      a.ws.part[(long long)(row0 + my_row) * a.parts + blockIdx.x - a.share.cta(block * a.groups)] = p;
+    }
+  }
+  // copies that a wait gave up on land before the CTA exits
+  if (VEC && *(volatile int*)&aborted != 0) {
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < kWaitLimitNs / 20) {
+    }
+  }
+}
+
+// ------------------------------------------------------------------ choosing the best of a list
+namespace {
+
+// The n-th largest of some keys, of which there are at least n, by bisection between their
+// smallest lo and largest hi (of a lane); the bisection stops early at a value that n to
+// `enough` keys reach.  count(mid): the lane's number of keys >= mid.
+template <typename Count>
+__device__ __forceinline__ uint32_t warp_kth(uint32_t lo, uint32_t hi, int n, int enough, Count count) {
+  lo = __reduce_min_sync(kAllLanes, lo);
+  hi = __reduce_max_sync(kAllLanes, hi);
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+    const int c = __reduce_add_sync(kAllLanes, count(mid));
+    if (c >= n) {
+      lo = mid;
+      if (c <= enough) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return lo;
+}
+
+// The n largest of the keys key(0..N-1) (n <= N), the lowest positions among equals:
+// emit(slot, position, key) with ascending positions.
+template <typename Key, typename Emit>
+__device__ __forceinline__ void warp_top(int N, int n, Key key, Emit emit) {
+  const int lane = threadIdx.x & 31;
+  uint32_t lo = 0xffffffffu, hi = 0;
+  for (int i = lane; i < N; i += 32) {
+    const uint32_t k = key(i);
+    lo = min(lo, k);
+    hi = max(hi, k);
+  }
+  const uint32_t T = warp_kth(lo, hi, n, n, [&](uint32_t mid) {
+    int c = 0;
+    for (int i = lane; i < N; i += 32) c += key(i) >= mid;
+    return c;
+  });
+  int above = 0;
+  for (int i = lane; i < N; i += 32) above += key(i) > T;
+  int ties = n - __reduce_add_sync(kAllLanes, above), at = 0;
+  for (int i0 = 0; i0 < N && at < n; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t k = i < N ? key(i) : 0u;
+    const uint32_t before = (1u << lane) - 1u;
+    const uint32_t same = __ballot_sync(kAllLanes, i < N && k == T);
+    const bool tie = ((same >> lane) & 1u) && __popc(same & before) < ties;
+    const uint32_t take = __ballot_sync(kAllLanes, (i < N && k > T) || tie);
+    if ((take >> lane) & 1u) emit(at + __popc(take & before), i, k);
+    at += __popc(take);
+    ties -= min(ties, __popc(same));
+  }
+  __syncwarp();
+}
+
+__device__ __forceinline__ unsigned long long entry_key(uint32_t key, int token) {
+  return ((unsigned long long)key << 32) | (unsigned long long)(0xFFFFFFFFu - (uint32_t)token);
+}
+
+// The finishing warp's own shared memory.
+struct RowScratch {
+  unsigned long long* list;  // [kBeamListCap] candidates
+  int* quarters;             // [kBeamListCap] 4 group + quarter
+  int* count;
+};
+
+// The row's `select` best logits by exact counting, however many are equal or crowd together
+// in a few groups, into w.list.  The `select` best groups by (maximum, lowest group) hold
+// them: a logit outside is beaten by one in each of those.
+template <typename T, bool MIX>
+__device__ __noinline__ void row_best_exact(const BeamSelectArgs& a, const T* logits, const Shared<T>& sh,
+                                            const float4* tops, const RowScratch& w) {
+  const int n_groups = min(a.select, a.groups);
+  warp_top(a.groups, n_groups,
+           [&](int i) {
+             const float4 t = __ldg(tops + i);
+             return ordered_u32(fmax_nan(fmax3_nan(t.x, t.y, t.z), t.w));
+           },
+           [&](int slot, int i, uint32_t) { w.quarters[slot] = i; });
+  // the groups ascend, so positions ascend with the tokens; only the last group can be short
+  const int last = a.V - w.quarters[n_groups - 1] * kBeamGroup;
+  const int total = (n_groups - 1) * kBeamGroup + min(kBeamGroup, last);
+  auto token = [&](int p) { return w.quarters[p / kBeamGroup] * kBeamGroup + p % kBeamGroup; };
+  warp_top(total, a.select, [&](int p) { return ordered_u32(mixed_logit<T, MIX>(logits, sh, token(p))); },
+           [&](int slot, int p, uint32_t k) { w.list[slot] = entry_key(k, token(p)); });
+}
+
+// A bound that at least n of the maxima top[0..3] of all lanes reach (the n-th largest, or a
+// little less: reading a few logits more takes less time than more bisection); 0 marks a
+// missing one, and 0 is returned when fewer than n are there.
+__device__ __forceinline__ uint32_t warp_bound(const uint32_t (&top)[4], int n) {
+  uint32_t lo = 0xffffffffu, hi = 0;
+  int some = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    lo = min(lo, top[r] == 0 ? 0xffffffffu : top[r]);
+    hi = max(hi, top[r]);
+    some += top[r] != 0;
+  }
+  if (__reduce_add_sync(kAllLanes, some) < n) return 0;
+  return warp_kth(lo, hi, n, n + 2 + n / 4, [&](uint32_t mid) {
+    return (top[0] >= mid) + (top[1] >= mid) + (top[2] >= mid) + (top[3] >= mid);
+  });
+}
+
+// Four logits of a lane from a quarter; -inf past V.  The loads of the logits and of what they
+// share leave together, before the first of them is used (volatile: in the order written), since
+// each may take a microsecond to come.
+template <typename T, bool MIX, bool VEC>
+__device__ __forceinline__ void load_quarter(const BeamSelectArgs& a, const T* logits, const Shared<T>& sh, int quarter,
+                                             int lane, float2 (&x)[2]) {
+  const int v = (quarter >> 2) * kBeamGroup + quarter_offset<VEC>(quarter & 3, lane, 0);
+  if constexpr (VEC) {
+    const int u = v < a.V ? v : 0;
+    Raw4<T> p, b;
+    Raw4<float> pr;
+    p.load(logits + u);
+    if constexpr (MIX) {
+      b.load((sh.base != nullptr ? sh.base : logits) + u);
+      if (sh.prior != nullptr) pr.load(sh.prior + u);
+    }
+    p.unpack(x);
+    if constexpr (MIX) {
+      float2 y[2];
+      if (sh.base != nullptr) {
+        b.unpack(y);
+        x[0] = add2(y[0], x[0]), x[1] = add2(y[1], x[1]);
+      }
+      if (sh.prior != nullptr) {
+        const float2 nb = make_float2(sh.nbeta, sh.nbeta);
+        pr.unpack(y);
+        x[0] = add2(x[0], mul2(nb, y[0])), x[1] = add2(x[1], mul2(nb, y[1]));
+      }
+    }
+    if (v >= a.V) x[0] = x[1] = make_float2(neg_inf(), neg_inf());
+  } else {
+    x[0].x = v < a.V ? mixed_logit<T, MIX>(logits, sh, v) : neg_inf();
+    x[0].y = v + 32 < a.V ? mixed_logit<T, MIX>(logits, sh, v + 32) : neg_inf();
+    x[1].x = v + 64 < a.V ? mixed_logit<T, MIX>(logits, sh, v + 64) : neg_inf();
+    x[1].y = v + 96 < a.V ? mixed_logit<T, MIX>(logits, sh, v + 96) : neg_inf();
+  }
+}
+
+// take(x, quarter) for each listed quarter.
+template <typename T, bool MIX, bool VEC, typename Take>
+__device__ __forceinline__ void each_quarter(const BeamSelectArgs& a, const T* logits, const Shared<T>& sh,
+                                             const int* quarters, int n_list, Take take) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int i = 0; i < n_list; i += 2) {  // two in flight
+    float2 x[2], y[2];
+    const int p = quarters[i], q = quarters[min(i + 1, n_list - 1)];
+    load_quarter<T, MIX, VEC>(a, logits, sh, p, lane, x);
+    load_quarter<T, MIX, VEC>(a, logits, sh, q, lane, y);
+    take(x, p);
+    if (i + 1 < n_list) take(y, q);
+  }
+}
+
+// The row's `select` best logits or a few more, in any order, into w.list; returns their
+// number.
+template <typename T, bool MIX, bool VEC>
+__device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits, const Shared<T>& sh,
+                                        const float4* tops, const RowScratch& w) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t none = ordered_u32(neg_inf());
+  // A bound that `select` logits reach: from 128 maxima over the quarters of the groups
+  // i, i + 32, ..., or, where there are hardly as many quarters as candidates (a small
+  // vocabulary), over the logits themselves.
+  const bool few = 4 * a.groups < 2 * a.select;
+  uint32_t top[4] = {0, 0, 0, 0};
+  if (!few) {
+#pragma unroll 5
+    for (int i = lane; i < a.groups; i += 32) {
+      const float4 t = __ldg(tops + i);
+      top[0] = max(top[0], ordered_u32(t.x)), top[1] = max(top[1], ordered_u32(t.y));
+      top[2] = max(top[2], ordered_u32(t.z)), top[3] = max(top[3], ordered_u32(t.w));
+    }
+  } else {
+    for (int i = lane; i < 4 * a.groups; i += 32) w.quarters[i] = i;  // at most 2 select of them
+    __syncwarp();
+    each_quarter<T, MIX, VEC>(a, logits, sh, w.quarters, 4 * a.groups, [&](const float2(&x)[2], int) {
+      top[0] = max(top[0], ordered_u32(x[0].x)), top[1] = max(top[1], ordered_u32(x[0].y));
+      top[2] = max(top[2], ordered_u32(x[1].x)), top[3] = max(top[3], ordered_u32(x[1].y));
+    });
+  }
+  uint32_t bound = warp_bound(top, a.select);
+  // Too little above -inf: take all that is, and the lowest masked tokens for the rest.
+  const bool fill = bound <= none;
+  if (fill) bound = none + 1;
+  const float floor = ordered_u32_to_float(bound);
+  int n_list = 4 * a.groups;
+  if (!few) {
+    if (lane == 0) *w.count = 0;
+    __syncwarp();
+#pragma unroll 1
+    for (int i = lane; i < a.groups; i += 32) {
+      const float4 t = __ldg(tops + i);
+      // NaN counts as above every bound
+      uint32_t reach = (t.x < floor ? 0u : 1u) | (t.y < floor ? 0u : 2u) | (t.z < floor ? 0u : 4u) | (t.w < floor ? 0u : 8u);
+#pragma unroll 1
+      for (; reach != 0; reach &= reach - 1) {
+        const int slot = atomicAdd(w.count, 1);
+        if (slot < kBeamListCap) w.quarters[slot] = 4 * i + __ffs((int)reach) - 1;
+      }
+    }
+    __syncwarp();
+    n_list = *w.count;
+    __syncwarp();
+  }
+  if (lane == 0) *w.count = 0;
+  __syncwarp();
+  if (n_list <= kBeamListCap) {
+    each_quarter<T, MIX, VEC>(a, logits, sh, w.quarters, n_list, [&](const float2(&x)[2], int q) {
+      uint32_t reach = (x[0].x < floor ? 0u : 1u) | (x[0].y < floor ? 0u : 2u) | (x[1].x < floor ? 0u : 4u) |
+                       (x[1].y < floor ? 0u : 8u);
+#pragma unroll 1
+      for (; reach != 0; reach &= reach - 1) {
+        const int j = __ffs((int)reach) - 1;
+        const float y = j & 2 ? (j & 1 ? x[1].y : x[1].x) : (j & 1 ? x[0].y : x[0].x);
+        const int slot = atomicAdd(w.count, 1);
+        if (slot < kBeamListCap) w.list[slot] = entry_key(ordered_u32(y), (q >> 2) * kBeamGroup + quarter_offset<VEC>(q & 3, lane, j));
+      }
+    });
+    __syncwarp();
+    int c = *w.count;
+    __syncwarp();
+    if (fill && c < a.select) {
+      // at most c of the first select + c tokens are not masked
+#pragma unroll 1
+      for (int v0 = 0; v0 < a.V && c < a.select; v0 += 32) {
+        const int v = v0 + lane;
+        const bool masked = v < a.V && mixed_logit<T, MIX>(logits, sh, v) == neg_inf();
+        const uint32_t take = __ballot_sync(kAllLanes, masked);
+        const int slot = c + __popc(take & ((1u << lane) - 1u));
+        if (masked) w.list[slot] = entry_key(none, v);  // slot < select + 32 <= kBeamListCap
+        c += __popc(take);
+      }
+      __syncwarp();
+    }
+    if (c >= a.select && c <= kBeamListCap) return c;
+  }
+  row_best_exact<T, MIX>(a, logits, sh, tops, w);
+  return a.select;
+}
+
+// Score of a logit in a row with (m, cum - log S) = st.
+__device__ __forceinline__ float row_score(float x, float2 st) { return x == neg_inf() ? neg_inf() : (x - st.x) + st.y; }
+
+// A candidate: (score, beam) and (x, token), both in the order in which larger is better.
+struct Candidate {
+  unsigned long long rank, within;
+};
+
+// The shared memory of a finishing CTA.
+struct FinishScratch {
+  float2* stat;      // [beams] maximum, cum - log S
+  uint32_t* value;   // [values] scores of maxima
+  Candidate* list;   // [kBeamFinishCap]
+  int2* quarters;    // [kBeamFinishCap] (beam, 4 group + quarter)
+  // for counting exactly: the beams' lists
+  BeamEntry* entries;  // [beams * select]
+  uint32_t* score;     // [beams * select]
+  char* rows;          // a RowScratch for each warp
+};
+
+template <typename T>
+__device__ __forceinline__ Shared<T> shared_terms(const BeamSelectArgs& a, int seq, bool mix) {
+  Shared<T> sh{nullptr, nullptr, 0.0f};
+  if (mix) {
+    if (a.base != nullptr) sh.base = static_cast<const T*>(a.base) + (long long)seq * a.ld_base;
+    if (a.prior != nullptr) sh.prior = a.prior, sh.nbeta = -__ldg(a.beta);
+  }
+  return sh;
+}
+
+// The selection beam by beam: each one's `select` best candidates, then the best of those.
+// However many scores are equal, masked, or crowd together.
+template <typename T, bool MIX, bool VEC>
+__device__ __noinline__ void finish_exact(const BeamSelectArgs& a, const FinishScratch& f) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = blockDim.x >> 5;
+  const int seq = blockIdx.x, n = a.select, total = a.beams * n;
+  RowScratch w;
+  w.list = reinterpret_cast<unsigned long long*>(f.rows) + warp * kBeamListCap;
+  w.quarters = reinterpret_cast<int*>(f.rows + n_warps * kBeamListCap * 8) + warp * kBeamListCap;
+  w.count = reinterpret_cast<int*>(f.rows + n_warps * kBeamListCap * 12) + warp;
+  const Shared<T> sh = shared_terms<T>(a, seq, MIX);
+#pragma unroll 1
+  for (int k = warp; k < a.beams; k += n_warps) {
+    const int row = seq * a.beams + k;
+    BeamEntry* out = f.entries + k * n;
+    const float2 st = f.stat[k];
+    if (a.finished != nullptr && a.finished[row] != 0) {
+      // one live candidate, the padding token; then the lowest other tokens at -inf
+      for (int i = lane; i < n; i += 32) {
+        out[i] = i == 0 ? BeamEntry{0.0f, a.pad_token} : BeamEntry{neg_inf(), i - 1 + (i - 1 >= a.pad_token)};
+        f.score[k * n + i] = ordered_u32(row_score(out[i].x, st));
+      }
+      continue;
+    }
+    const int c = row_best<T, MIX, VEC>(a, static_cast<const T*>(a.logits) + (long long)row * a.ld, sh,
+                                        a.ws.group_top + (long long)row * a.groups, w);
+    __syncwarp();
+    for (int i = lane; i < c; i += 32) {
+      const unsigned long long mine = w.list[i];
+      int rank = 0;
+      for (int j = 0; j < c; ++j) rank += w.list[j] > mine;
+      if (rank < n) {
+        const float x = ordered_u32_to_float((uint32_t)(mine >> 32));
+        out[rank] = BeamEntry{x, (int)(0xFFFFFFFFu - (uint32_t)mine)};
+        f.score[k * n + rank] = ordered_u32(row_score(x, st));
+      }
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp != 0) return;
+  // (the warp's list is free again: at most kBeamMax positions and their keys)
+  int* pos = w.quarters;
+  uint32_t* pos_key = reinterpret_cast<uint32_t*>(w.list);
+  warp_top(total, n, [&](int i) { return f.score[i]; },
+           [&](int slot, int i, uint32_t k) { pos[slot] = i, pos_key[slot] = k; });
+  for (int i = lane; i < n; i += 32) {
+    // positions ascend with the slots, so equal scores keep the order of their slots
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += pos_key[j] > pos_key[i] || (pos_key[j] == pos_key[i] && j < i);
+    const long long o = (long long)seq * n + rank;
+    a.parents[o] = pos[i] / n;
+    a.tokens[o] = f.entries[pos[i]].token;
+    a.scores[o] = ordered_u32_to_float(pos_key[i]);
+  }
+}
+
+}  // namespace
+
+// A CTA per sequence; `finish_split` warps share a beam's groups.  The scores of group maxima,
+// over all beams, bound the sequence's `select` best scores from below; few quarters reach the
+// bound (about `select` of all beams together), and only they are read again, a warp each.
+// Where the bound says little (masked rows, many equal scores, more candidates than the list
+// holds) the CTA counts exactly, beam by beam.
+template <typename T, bool MIX, bool VEC>
+__global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(const BeamSelectArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ int n_found, n_quarters;
+  __shared__ uint32_t bound_key;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = blockDim.x >> 5;
+  const int seq = blockIdx.x, n = a.select;
+  const int split = a.finish_split;
+  const int at_once = n_warps / split, part = warp % split;
+  const int per_lane = a.finish_values;  // maxima a lane offers: 1 or 4
+  const int values = a.beams * split * 32 * per_lane;
+  FinishScratch f;
+  f.stat = reinterpret_cast<float2*>(smem);
+  char* rest = smem + (a.beams * 8 + 15) / 16 * 16;
+  f.list = reinterpret_cast<Candidate*>(rest);
+  f.quarters = reinterpret_cast<int2*>(f.list + kBeamFinishCap);
+  f.value = reinterpret_cast<uint32_t*>(f.quarters + kBeamFinishCap);
+  f.rows = rest;  // an exact count starts over, but for the rows' statistics
+  f.entries = reinterpret_cast<BeamEntry*>(rest + n_warps * kBeamRowScratch);
+  f.score = reinterpret_cast<uint32_t*>(f.entries + a.beams * n);
+  if (threadIdx.x == 0) n_found = n_quarters = 0;
+  const int blocks_per_seq = (a.beams + a.scan_rows - 1) / a.scan_rows;
+  pdl_wait();
+#pragma unroll 1
+  for (int k = warp / split; k < a.beams; k += at_once) {
+    const int row = seq * a.beams + k;
+    const bool done = a.finished != nullptr && a.finished[row] != 0;
+    const float cum = __ldg(a.cum + row);
+    float2 st = make_float2(0.0f, cum);
+    float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
+    if (!done) {
+      const int unit = (seq * blocks_per_seq + k / a.scan_rows) * a.groups;
+      const int parts = a.share.cta(unit + a.groups - 1) - a.share.cta(unit) + 1;
+      const float2* row_part = a.ws.part + (long long)row * a.parts;
+      float2 p = __ldcg(row_part + min(lane, parts - 1));
+      const float4* tops = a.ws.group_top + (long long)row * a.groups;
+#pragma unroll 5
+      for (int i = part * 32 + lane; i < a.groups; i += 32 * split) {
+        const float4 t = __ldg(tops + i);
+        top[0] = fmax_nan(top[0], t.x), top[1] = fmax_nan(top[1], t.y);
+        top[2] = fmax_nan(top[2], t.z), top[3] = fmax_nan(top[3], t.w);
+      }
+      if (lane >= parts) p = make_float2(neg_inf(), 0.0f);
+#pragma unroll 1
+      for (int i = lane + 32; i < parts; i += 32) p = softmax_join(p, __ldcg(row_part + i));
+#pragma unroll 1
+      for (int o = 16; o > 0; o >>= 1) {
+        const float2 q = make_float2(__shfl_down_sync(kAllLanes, p.x, o), __shfl_down_sync(kAllLanes, p.y, o));
+        p = softmax_join(p, q);
+      }
+      st = make_float2(__shfl_sync(kAllLanes, p.x, 0), cum - logf(__shfl_sync(kAllLanes, p.y, 0)));
+    } else if (part == 0 && lane == 0) {
+      top[0] = 0.0f;  // the padding token
+    }
+    if (part == 0 && lane == 0) f.stat[k] = st;
+    uint32_t* value = f.value + ((k * split + part) * 32 + lane) * per_lane;
+    if (per_lane == 1) {
+      value[0] = ordered_u32(row_score(fmax_nan(fmax3_nan(top[0], top[1], top[2]), top[3]), st));
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int v = v0 + j * 32 + lane;
-        x[j] = v < a.V ? mixed_logit<T, MIX>(logits, base, a.prior, beta, v) : neg_inf();
+      for (int i = 0; i < 4; ++i) value[i] = ordered_u32(row_score(top[i], st));
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    // up to 16 of the values of a lane in registers, so that the bisection hardly waits
+    constexpr int R = 16;
+    uint32_t v[R], lo = 0xffffffffu, hi = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const bool some = lane + 32 * i < values;
+      v[i] = some ? f.value[lane + 32 * i] : 0u;
+      lo = min(lo, some ? v[i] : 0xffffffffu);
+      hi = max(hi, v[i]);
+    }
+    for (int i = lane + 32 * R; i < values; i += 32) {
+      lo = min(lo, f.value[i]);
+      hi = max(hi, f.value[i]);
+    }
+    const uint32_t key = warp_kth(lo, hi, n, n + 2 + n / 4, [&](uint32_t mid) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) c += v[i] >= mid;
+      for (int i = lane + 32 * R; i < values; i += 32) c += f.value[i] >= mid;
+      return c;
+    });
+    if (lane == 0) bound_key = key;
+  }
+  __syncthreads();
+  const uint32_t none = ordered_u32(neg_inf());
+  // With too little above -inf: all that is, and masked tokens for the rest.  (Above the largest
+  // number there is NaN only, which says nothing of what else there is.)
+  const bool fill = bound_key <= none, exact = bound_key == 0xffffffffu;
+  const uint32_t key = fill ? none + 1 : bound_key;
+  if (!exact) {
+    const float bound = ordered_u32_to_float(key);
+    auto found = [&](int k, float x, float score, int token) {
+      const int slot = atomicAdd(&n_found, 1);
+      if (slot < kBeamFinishCap)
+        f.list[slot] = {((unsigned long long)ordered_u32(score) << 32) | (0xFFFFFFFFu - (uint32_t)k),
+                        entry_key(ordered_u32(x), token)};
+    };
+#pragma unroll 1
+    for (int k = warp / split; k < a.beams; k += at_once) {
+      const int row = seq * a.beams + k;
+      const float2 st = f.stat[k];
+      if (a.finished != nullptr && a.finished[row] != 0) {
+        if (part == 0 && lane == 0 && !(st.y < bound)) found(k, 0.0f, st.y, a.pad_token);
+        continue;
+      }
+      // few lanes hold a maximum that reaches the bound
+      const uint32_t* value = f.value + ((k * split + part) * 32 + lane) * per_lane;
+      if (value[0] < key && (per_lane == 1 || max(max(value[1], value[2]), value[3]) < key)) continue;
+      const float4* tops = a.ws.group_top + (long long)row * a.groups;
+#pragma unroll 5
+      for (int i = part * 32 + lane; i < a.groups; i += 32 * split) {
+        const float4 t = __ldg(tops + i);
+        // (a NaN reaches every bound)
+        if (row_score(fmax_nan(fmax3_nan(t.x, t.y, t.z), t.w), st) < bound) continue;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          if (row_score(q & 2 ? (q & 1 ? t.w : t.z) : (q & 1 ? t.y : t.x), st) < bound) continue;
+          const int slot = atomicAdd(&n_quarters, 1);
+          if (slot < kBeamFinishCap) f.quarters[slot] = make_int2(k, 4 * i + q);
+        }
       }
     }
-    float top = fmax_nan(fmax3_nan(x[0], x[1], x[2]), fmax3_nan(x[3], x[4], x[5]));
-    top = warp_max_nan(fmax3_nan(top, x[6], x[7]));
-    if (top > m) {
-      s *= __expf(m - top);  // m = -inf: s is 0 and stays 0
-      m = top;
+    __syncthreads();
+    const Shared<T> sh = shared_terms<T>(a, seq, MIX);
+    const int n_list = min(n_quarters, kBeamFinishCap);
+#pragma unroll 1
+    for (int i = warp; i < n_list; i += n_warps) {
+      const int k = f.quarters[i].x, q = f.quarters[i].y;
+      const float2 st = f.stat[k];
+      float2 x[2];
+      load_quarter<T, MIX, VEC>(a, static_cast<const T*>(a.logits) + (long long)(seq * a.beams + k) * a.ld, sh, q, lane, x);
+      if (row_score(fmax_nan(fmax3_nan(x[0].x, x[0].y, x[1].x), x[1].y), st) < bound) continue;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
+        const float y = j & 2 ? (j & 1 ? x[1].y : x[1].x) : (j & 1 ? x[0].y : x[0].x);
+        const float score = row_score(y, st);
+        if (!(score < bound)) found(k, y, score, (q >> 2) * kBeamGroup + quarter_offset<VEC>(q & 3, lane, j));
+      }
     }
-    const float ref = m == neg_inf() ? 0.0f : m;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s += __expf(x[j] - ref);
-    if (lane == 0) a.ws.group_key[(long long)row * a.groups + g] = ordered_u32(top);
   }
-  s = warp_sum(s);
-  if (lane == 0) warp_part[warp] = make_float2(m, s);
   __syncthreads();
-  if (threadIdx.x == 0) {
-    float2 p = warp_part[0];
-    for (int w = 1; w < kBeamThreads / 32; ++w) p = softmax_join(p, warp_part[w]);
-    a.ws.part[(long long)row * a.slices + slice] = p;
-  }
-}
-
-// Dynamic shared memory: keys [max(groups, select * kBeamGroup)] uint32.
-template <typename T, bool MIX>
-__global__ void __launch_bounds__(kBeamThreads) beam_row_kernel(const BeamSelectArgs a) {
-  extern __shared__ uint32_t keys[];
-  __shared__ uint32_t shared4[4];
-  __shared__ int groups[kBeamMax], pos[kBeamMax];
-  __shared__ unsigned long long best[kBeamMax];
-  const int row = blockIdx.x, t = threadIdx.x;
-  pdl_wait();
-  BeamEntry* out = a.ws.best + (long long)row * a.select;
-  if (a.finished != nullptr && a.finished[row] != 0) {
-    // one live candidate, the padding token; then the lowest other tokens at -inf
-    for (int i = t; i < a.select; i += kBeamThreads) {
-      const int rest = i - 1 + (i - 1 >= a.pad_token);
-      out[i] = i == 0 ? BeamEntry{0.0f, a.pad_token} : BeamEntry{neg_inf(), rest};
+  if (fill && n_found < n) {
+    // The rest are masked tokens, the lowest of the lowest beam.  A beam whose own score is
+    // not finite has other candidates at -inf, which an exact count sorts out.
+    const int row = seq * a.beams;
+    const bool done = a.finished != nullptr && a.finished[row] != 0;
+    if (warp == 0 && fabsf(f.stat[0].y) < __int_as_float(0x7f800000)) {
+      const Shared<T> sh = shared_terms<T>(a, seq, MIX);
+      const T* logits = static_cast<const T*>(a.logits) + (long long)row * a.ld;
+      int c = n_found;
+#pragma unroll 1
+      for (int v0 = 0; v0 < a.V && c < n; v0 += 32) {
+        const int v = v0 + lane;
+        const bool masked = v < a.V && (done ? v != a.pad_token : mixed_logit<T, MIX>(logits, sh, v) == neg_inf());
+        const uint32_t take = __ballot_sync(kAllLanes, masked);
+        // at most select + 31 candidates
+        if (masked) f.list[c + __popc(take & ((1u << lane) - 1u))] = {((unsigned long long)none << 32) | 0xFFFFFFFFu,
+                                                                    entry_key(none, v)};
+        c += __popc(take);
+      }
+      if (lane == 0) n_found = c;
     }
-    if (t == 0) a.ws.stat[row] = make_float2(0.0f, a.cum[row]);
+    __syncthreads();
+  }
+  const int c = n_found;
+  if (exact || n_quarters > kBeamFinishCap || c < n || c > kBeamFinishCap) {
+    finish_exact<T, MIX, VEC>(a, f);
     return;
   }
-  if (t == 0) {
-    const float2* part = a.ws.part + (long long)row * a.slices;
-    float2 p = part[0];
-    for (int i = 1; i < a.slices; ++i) p = softmax_join(p, part[i]);
-    a.ws.stat[row] = make_float2(p.x, a.cum[row] - logf(p.y));
-  }
-  for (int g = t; g < a.groups; g += kBeamThreads) keys[g] = a.ws.group_key[(long long)row * a.groups + g];
-  __syncthreads();
-  const int n_groups = min(a.select, a.groups);
-  block_top_positions(keys, a.groups, n_groups, groups, shared4);
-  const T* logits = static_cast<const T*>(a.logits) + (long long)row * a.ld;
-  const T* base = nullptr;
-  float beta = 0.0f;
-  if constexpr (MIX) {
-    if (a.base != nullptr) base = static_cast<const T*>(a.base) + (long long)(row / a.beams) * a.ld_base;
-    if (a.prior != nullptr) beta = __ldg(a.beta);
-  }
-  // the groups ascend, so positions ascend with the tokens; only the last group can be
-  // short, and it is the last one here
-  int total = 0;
-  for (int i = 0; i < n_groups; ++i) {
-    const int v0 = groups[i] * kBeamGroup, len = min(kBeamGroup, a.V - v0);
-    for (int j = t; j < len; j += kBeamThreads)
-      keys[total + j] = ordered_u32(mixed_logit<T, MIX>(logits, base, a.prior, beta, v0 + j));
-    total += len;
-  }
-  __syncthreads();
-  block_top_positions(keys, total, a.select, pos, shared4);
-  if (t < a.select) {
-    const int p = pos[t];
-    const int token = groups[p / kBeamGroup] * kBeamGroup + p % kBeamGroup;
-    best[t] = ((unsigned long long)keys[p] << 32) | (unsigned long long)(0xFFFFFFFFu - (uint32_t)token);
-  }
-  __syncthreads();
-  if (t < a.select) {
+  for (int i = threadIdx.x; i < c; i += blockDim.x) {
+    const Candidate mine = f.list[i];
     int rank = 0;
-    for (int i = 0; i < a.select; ++i) rank += best[i] > best[t];
-    out[rank] = BeamEntry{ordered_u32_to_float((uint32_t)(best[t] >> 32)),
-                          (int)(0xFFFFFFFFu - (uint32_t)(best[t] & 0xFFFFFFFFull))};
+#pragma unroll 2
+    for (int j = 0; j < c; ++j) {
+      const Candidate other = f.list[j];
+      rank += other.rank > mine.rank || (other.rank == mine.rank && other.within > mine.within);
+    }
+    if (rank < n) {
+      const long long o = (long long)seq * n + rank;
+      a.parents[o] = (int)(0xFFFFFFFFu - (uint32_t)mine.rank);
+      a.tokens[o] = (long long)(0xFFFFFFFFu - (uint32_t)mine.within);
+      a.scores[o] = ordered_u32_to_float((uint32_t)(mine.rank >> 32));
+    }
   }
 }
 
-// Dynamic shared memory: keys [beams * select] uint32.
-__global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const BeamSelectArgs a) {
-  extern __shared__ uint32_t keys[];
-  __shared__ uint32_t shared4[4];
-  __shared__ int pos[kBeamMax];
-  __shared__ unsigned long long best[kBeamMax];
-  const int seq = blockIdx.x, t = threadIdx.x;
-  pdl_wait();
-  const BeamEntry* lists = a.ws.best + (long long)seq * a.beams * a.select;
-  const int total = a.beams * a.select;
-  for (int i = t; i < total; i += kBeamThreads) {
-    const float2 st = a.ws.stat[seq * a.beams + i / a.select];
-    const float x = lists[i].x;
-    keys[i] = ordered_u32(x == neg_inf() ? neg_inf() : (x - st.x) + st.y);
-  }
-  __syncthreads();
-  block_top_positions(keys, total, a.select, pos, shared4);
-  if (t < a.select)
-    best[t] = ((unsigned long long)keys[pos[t]] << 32) | (unsigned long long)(0xFFFFFFFFu - (uint32_t)pos[t]);
-  __syncthreads();
-  if (t < a.select) {
-    int rank = 0;
-    for (int i = 0; i < a.select; ++i) rank += best[i] > best[t];
-    const long long o = (long long)seq * a.select + rank;
-    a.parents[o] = pos[t] / a.select;
-    a.tokens[o] = lists[pos[t]].token;
-    a.scores[o] = ordered_u32_to_float(keys[pos[t]]);
-  }
-}
-
-template __global__ void beam_scan_kernel<float, false, false>(const BeamSelectArgs);
-template __global__ void beam_scan_kernel<float, false, true>(const BeamSelectArgs);
-template __global__ void beam_scan_kernel<float, true, false>(const BeamSelectArgs);
-template __global__ void beam_scan_kernel<float, true, true>(const BeamSelectArgs);
-template __global__ void beam_scan_kernel<__nv_bfloat16, false, false>(const BeamSelectArgs);
-template __global__ void beam_scan_kernel<__nv_bfloat16, false, true>(const BeamSelectArgs);
-template __global__ void beam_scan_kernel<__nv_bfloat16, true, false>(const BeamSelectArgs);
-template __global__ void beam_scan_kernel<__nv_bfloat16, true, true>(const BeamSelectArgs);
-template __global__ void beam_row_kernel<float, false>(const BeamSelectArgs);
-template __global__ void beam_row_kernel<float, true>(const BeamSelectArgs);
-template __global__ void beam_row_kernel<__nv_bfloat16, false>(const BeamSelectArgs);
-template __global__ void beam_row_kernel<__nv_bfloat16, true>(const BeamSelectArgs);
+#define DELS_BEAM_KERNELS(T, MIX, VEC)                                    \
+  template __global__ void beam_scan_kernel<T, MIX, VEC>(const BeamSelectArgs); \
+  template __global__ void beam_finish_kernel<T, MIX, VEC>(const BeamSelectArgs);
+DELS_BEAM_KERNELS(float, false, false)
+DELS_BEAM_KERNELS(float, false, true)
+DELS_BEAM_KERNELS(float, true, false)
+DELS_BEAM_KERNELS(float, true, true)
+DELS_BEAM_KERNELS(__nv_bfloat16, false, false)
+DELS_BEAM_KERNELS(__nv_bfloat16, false, true)
+DELS_BEAM_KERNELS(__nv_bfloat16, true, false)
+DELS_BEAM_KERNELS(__nv_bfloat16, true, true)
+#undef DELS_BEAM_KERNELS
 
 // --------------------------------------------------------------------------------
 // Reordering.  dst[b, j] = src[b, parents[b, j]] for every state.  A tile is one piece of

@@ -7,9 +7,13 @@
 namespace dels {
 
 constexpr int kBeamMax = 64;         // beams of a sequence, read or selected
-constexpr int kBeamGroup = 256;      // logits of a group, the unit a warp scans at a time
-constexpr int kBeamMaxGroups = 2048; // groups of a row: at most 524288 logits
-constexpr int kBeamThreads = 256;
+constexpr int kBeamGroup = 512;      // logits of a group, the unit a warp scans at a time
+constexpr int kBeamScanWarps = 4;    // most warps of a scanning CTA
+constexpr int kBeamScanRows = 8;     // most rows a scanning CTA takes through the logits they share
+constexpr int kBeamFinishWarps = 16; // most warps of a sequence's finishing CTA
+constexpr int kBeamFinishCap = 256;  // quarter groups or candidates it lists before it counts exactly
+constexpr int kBeamListCap = 192;    // counting exactly: quarter groups or logits a warp lists
+constexpr int kBeamRowScratch = kBeamListCap * 12 + 16;
 
 // One (value, token) entry of a row's list of best candidates.
 struct BeamEntry {
@@ -18,12 +22,22 @@ struct BeamEntry {
 };
 
 // Scratch of one selection.  A row is a beam of a sequence; its V logits are cut into
-// `groups` groups of kBeamGroup logits, and its scan into `slices` CTAs.
+// `groups` groups of kBeamGroup; see beam_scan_kernel for the parts.
 struct BeamScratch {
-  uint32_t* group_key;  // [rows][groups] ordered maxima
-  float2* part;         // [rows][slices] running maximum and sum of a slice
-  BeamEntry* best;      // [rows][select] the row's candidates, best first
-  float2* stat;         // [rows] maximum, cum - log(sum)
+  float4* group_top;  // [rows][groups] maxima of a group's quarters
+  float2* part;       // [rows][parts] running maximum and sum of a CTA's share of the row
+};
+
+// The scan's CTAs share out the units (all blocks' groups, in order) as evenly as they go: CTA
+// c takes [first(c), first(c + 1)), per of them or one more.
+struct ScanShare {
+  int per, more;  // the first `more` CTAs take per + 1
+  __host__ __device__ __forceinline__ int first(int c) const { return c * per + (c < more ? c : more); }
+  // the CTA that takes unit u
+  __host__ __device__ __forceinline__ int cta(int u) const {
+    const int cut = more * (per + 1);
+    return u < cut ? u / (per + 1) : more + (u - cut) / per;
+  }
 };
 
 struct BeamSelectArgs {
@@ -37,18 +51,47 @@ struct BeamSelectArgs {
   const uint8_t* finished;   // [rows] or null
   int pad_token;
   int n_seq, beams, select, V;
-  int groups, slices;
+  int groups, parts;
+  int scan_rows;             // rows that are scanned together (a block of rows)
+  int scan_ctas;
+  ScanShare share;
+  int finish_split;          // warps of the finishing CTA that share a beam
+  int finish_values;         // group maxima a lane of them offers for the bound
+  int slot_bytes;            // of its staging ring
+  int* status;               // device error word
   int* parents;              // [n_seq, select]
   long long* tokens;         // [n_seq, select]
   float* scores;             // [n_seq, select]
   BeamScratch ws;
 };
 
+// Warps that scan a group together, two rows (MIX) each, and teams of them in a CTA.
+__host__ __device__ __forceinline__ int scan_pairs(int rows) { return (rows + 1) / 2; }
+__host__ __device__ __forceinline__ int scan_teams(int rows) { return kBeamScanWarps / scan_pairs(rows); }
+
+// The scan's staging rings, one for each team: groups in flight.
+constexpr int beam_scan_depth(int elem, bool mix) { return mix ? (elem == 2 ? 3 : 2) : 6; }
+// Bytes of a slot: `rows` rows of a group, and the draft logits and prior they share.
+constexpr int beam_slot_bytes(int rows, int elem, bool mix) {
+  return rows * kBeamGroup * elem + (mix ? kBeamGroup * (elem + 4) : 0);
+}
+// Dynamic shared memory of beam_scan_kernel with VEC.
+inline int beam_scan_smem(int rows, int elem, bool mix) {
+  return scan_teams(rows) * beam_scan_depth(elem, mix) * beam_slot_bytes(rows, elem, mix);
+}
+constexpr int kBeamScanSmemMax = 65536;  // two rows of fp32: 4 teams x 2 slots x 8 KB
+
+// Dynamic shared memory of beam_finish_kernel.
+constexpr int beam_finish_smem(int beams, int select, int warps, int values) {
+  const int listing = kBeamFinishCap * 24 + values * 4;
+  const int exact = warps * kBeamRowScratch + beams * select * 12;
+  return (beams * 8 + 15) / 16 * 16 + (listing > exact ? listing : exact);
+}
+
 template <typename T, bool MIX, bool VEC>
 __global__ void beam_scan_kernel(const BeamSelectArgs a);
-template <typename T, bool MIX>
-__global__ void beam_row_kernel(const BeamSelectArgs a);
-__global__ void beam_merge_kernel(const BeamSelectArgs a);
+template <typename T, bool MIX, bool VEC>
+__global__ void beam_finish_kernel(const BeamSelectArgs a);
 
 // One state of the beams: rows x outer x inner contiguous bytes.
 struct BeamState {
@@ -64,6 +107,7 @@ struct BeamState {
 };
 
 constexpr int kBeamStatesPerLaunch = 32;
+constexpr int kBeamThreads = 256;
 
 struct BeamReorderArgs {
   BeamState st[kBeamStatesPerLaunch];

@@ -9,6 +9,7 @@ call.  There is deliberately no CPU or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -865,15 +866,37 @@ _FLOATS = {torch.bfloat16: _lib.DELS_DTYPE_BF16, torch.float32: _lib.DELS_DTYPE_
 
 def _require_float(name: str, t: torch.Tensor, ndim: int) -> int:
     """The DELS_DTYPE_* code of a bf16 or fp32 CUDA tensor."""
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dtype not in _FLOATS or t.dim() != ndim:
+    code = _FLOATS.get(t.dtype) if isinstance(t, torch.Tensor) and t.is_cuda else None
+    if code is None or t.dim() != ndim:
         raise ValueError(f"{name} must be a {ndim}-D bf16 or fp32 CUDA tensor; there is no CPU path")
-    return _FLOATS[t.dtype]
+    return code
 
 
 def _require_dense(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device} "
                          f"(got {t.dtype} {tuple(t.shape)} on {t.device}, stride {t.stride()})")
+
+
+# A draft step calls these operators on small tensors, where the host's part of a call is what
+# counts: addresses go to ctypes as plain integers, sizes of workspaces are asked for once.
+def _addr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@functools.lru_cache(maxsize=4096)
+def _bytes(query: str, *args: int) -> int:
+    return int(_lib.query(query, *args))
+
+
+def _stream_workspace(nbytes: int, device: torch.device, stream: int) -> Workspace:
+    """workspace() for a stream that is known already."""
+    ws = _ws_cache.get((device.index, stream))
+    return workspace(nbytes, device) if ws is None or ws.nbytes < nbytes else ws
 
 
 def quantize_rows_i8(
@@ -896,8 +919,8 @@ def quantize_rows_i8(
         scale = torch.empty(rows, dtype=torch.float32, device=dev)
     else:
         _require_dense("scale", scale, torch.float32, (rows,), dev)
-    _lib.call("dels_quantize_rows_i8", _ptr(x), code, _row_major("x", x), rows, K, _ptr(q), _row_major("q", q),
-              _ptr(scale), _stream(dev))
+    _lib.call("dels_quantize_rows_i8", _addr(x), code, _row_major("x", x), rows, K, _addr(q), _row_major("q", q),
+              _addr(scale), _raw_stream(dev))
     return q, scale
 
 
@@ -939,15 +962,16 @@ def linear_i8(
     rows, K = xq.shape
     _require_dense("x_scale", x_scale, torch.float32, (rows,), dev)
     N, out = _i8_operands(rows, K, dev, wq, w_scale, bias, out, out_dtype)
-    ws = workspace(_lib.DELS_WS_HEADER_BYTES, dev) if ws is None else ws
-    _lib.call("dels_linear_i8", _ptr(xq), _row_major("xq", xq), _ptr(x_scale), _ptr(wq), _row_major("wq", wq),
-              _ptr(w_scale), _ptr(bias), rows, K, N, _ptr(out), _FLOATS[out.dtype], _row_major("out", out), ws.ptr,
-              ws.nbytes, _stream(dev))
+    stream = _raw_stream(dev)
+    ws = _stream_workspace(_lib.DELS_WS_HEADER_BYTES, dev, stream) if ws is None else ws
+    _lib.call("dels_linear_i8", _addr(xq), _row_major("xq", xq), _addr(x_scale), _addr(wq), _row_major("wq", wq),
+              _addr(w_scale), _addr(bias), rows, K, N, _addr(out), _FLOATS[out.dtype], _row_major("out", out), ws.ptr,
+              ws.nbytes, stream)
     return out
 
 
 def linear_w8a8_workspace_bytes(rows: int, K: int) -> int:
-    return int(_lib.query("dels_linear_w8a8_workspace_bytes", rows, K))
+    return _bytes("dels_linear_w8a8_workspace_bytes", rows, K)
 
 
 def linear_w8a8(
@@ -969,10 +993,11 @@ def linear_w8a8(
     rows, K = x.shape
     N, out = _i8_operands(rows, K, dev, wq, w_scale, bias, out, x.dtype if out_dtype is None else out_dtype)
     need = linear_w8a8_workspace_bytes(rows, K)
-    ws = workspace(need, dev) if ws is None else ws.ensure(need)
-    _lib.call("dels_linear_w8a8", _ptr(x), code, _row_major("x", x), _ptr(wq), _row_major("wq", wq), _ptr(w_scale),
-              _ptr(bias), rows, K, N, _ptr(out), _FLOATS[out.dtype], _row_major("out", out), ws.ptr, ws.nbytes,
-              _stream(dev))
+    stream = _raw_stream(dev)
+    ws = _stream_workspace(need, dev, stream) if ws is None else ws.ensure(need)
+    _lib.call("dels_linear_w8a8", _addr(x), code, _row_major("x", x), _addr(wq), _row_major("wq", wq), _addr(w_scale),
+              _addr(bias), rows, K, N, _addr(out), _FLOATS[out.dtype], _row_major("out", out), ws.ptr, ws.nbytes,
+              stream)
     return out
 
 
@@ -1038,29 +1063,34 @@ def beam_select(
         _require_dense("out.parents", out.parents, torch.int32, (n_seq, n), dev)
         _require_dense("out.tokens", out.tokens, torch.int64, (n_seq, n), dev)
         _require_dense("out.scores", out.scores, torch.float32, (n_seq, n), dev)
-    need = _lib.query("dels_beam_select_workspace_bytes", n_seq, beams, n, V)
-    ws = workspace(need, dev) if ws is None else ws.ensure(need)
+    need = beam_select_workspace_bytes(n_seq, beams, n, V)
+    stream = _raw_stream(dev)
+    ws = _stream_workspace(need, dev, stream) if ws is None else ws.ensure(need)
     _lib.call(
-        "dels_beam_select", _ptr(logits), code, _row_major("logits", logits), _ptr(base),
-        0 if base is None else _row_major("base", base), _ptr(prior), _ptr(beta), _ptr(scores), _ptr(finished),
-        int(pad_token), n_seq, beams, n, V, _ptr(out.parents), _ptr(out.tokens), _ptr(out.scores), ws.ptr, ws.nbytes,
-        _stream(dev),
+        "dels_beam_select", _addr(logits), code, _row_major("logits", logits), _addr(base),
+        0 if base is None else _row_major("base", base), _addr(prior), _addr(beta), _addr(scores), _addr(finished),
+        int(pad_token), n_seq, beams, n, V, _addr(out.parents), _addr(out.tokens), _addr(out.scores), ws.ptr,
+        ws.nbytes, stream,
     )
     return out
 
 
 def beam_select_workspace_bytes(n_seq: int, beams: int, select: int, V: int) -> int:
-    return int(_lib.query("dels_beam_select_workspace_bytes", n_seq, beams, select, V))
+    return _bytes("dels_beam_select_workspace_bytes", n_seq, beams, select, V)
+
+
+@functools.lru_cache(maxsize=None)
+def _int64_array(n: int):
+    return ctypes.c_int64 * n
 
 
 def _beam_state(i: int, src: torch.Tensor, dst: torch.Tensor) -> tuple:
     """The dels_beam_state of one (src, dst) pair: rows of ``outer`` runs of contiguous bytes."""
     item = src.element_size()
     if src.is_contiguous() and dst.is_contiguous():
-        inner = 1
-        for n in src.shape[1:]:
-            inner *= n
-        return src.data_ptr(), dst.data_ptr(), inner * item, inner * item, 0, 0, 1, inner * item
+        # (by its size: the stride of a dimension of one row may be anything)
+        row = src.numel() // src.shape[0] * item if src.shape[0] else 0
+        return src.data_ptr(), dst.data_ptr(), row, row, 0, 0, 1, row
     shape, ss, ds = src.shape, src.stride(), dst.stride()
     inner, k = 1, src.dim() - 1
     while k >= 1 and (shape[k] == 1 or (ss[k] == inner and ds[k] == inner)):
@@ -1116,8 +1146,8 @@ def beam_reorder(
             raise ValueError(f"state {i}: {src.dtype} {tuple(src.shape)} -> {dst.dtype} {tuple(dst.shape)} does not "
                              f"match {n_seq} sequences of {beams} -> {n} beams")
         table.extend(_beam_state(i, src, dst))
-    _lib.call("dels_beam_reorder", (ctypes.c_int64 * len(table))(*table), len(states), _ptr(parents), n_seq,
-              int(beams), n, _ptr(status), _stream(dev))
+    _lib.call("dels_beam_reorder", _int64_array(len(table))(*table), len(states), _addr(parents), n_seq, int(beams), n,
+              _addr(status), _raw_stream(dev))
     return out
 
 

@@ -394,7 +394,7 @@ DELS_API int dels_linear_w8a8(const void* x, int x_dtype, int64_t ld_x, const in
  *   cum [n_seq, beams] fp32; finished bytes [n_seq, beams] or NULL.
  *   parents [n_seq, select] int32 (0..beams-1), tokens [n_seq, select] int64, scores
  *   [n_seq, select] fp32, which may be `cum` itself when select == beams.
- * 1 <= beams, select <= DELS_BEAM_MAX, select <= V <= DELS_BEAM_MAX_VOCAB;
+ * 1 <= beams, select <= DELS_BEAM_MAX, select <= V <= DELS_BEAM_MAX_VOCAB, at most 2^20 rows;
  * ws >= dels_beam_select_workspace_bytes(). */
 DELS_API size_t dels_beam_select_workspace_bytes(int n_seq, int beams, int select, int V);
 DELS_API int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const void* base, int64_t ld_base,

@@ -328,6 +328,19 @@ def test_reorder_many_states_and_transposed_rows(cuda_device):
     assert torch.equal(layered, want)
 
 
+def test_reorder_single_rows_of_wider_tensors(cuda_device):
+    """One sequence with one beam: the row stride of such a slice says nothing of its length."""
+    from dels_b200 import ops
+
+    dev = cuda_device
+    p = torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    wide = torch.randn(3, 50, device=dev)
+    assert ops._beam_state(0, wide[1:2, :7], wide[2:3, :7])[-1] == 28
+    out = torch.full((3, 50), 7.0, device=dev)
+    ops.beam_reorder([wide[1:2, :7]], p, beams=1, out=[out[1:2, 3:10]])
+    assert torch.equal(out[1, 3:10], wide[1, :7]) and (out[[0, 2]] == 7).all() and (out[1, 10:] == 7).all()
+
+
 def test_reorder_bad_parent_is_reported(cuda_device):
     from dels_b200 import _lib, ops
 
