@@ -216,6 +216,7 @@ cudaError_t set_smem(K kernel, int bytes) {
 }
 
 constexpr int kMaxSmem = 232448;
+static_assert(kBeamReorderSmem / kBeamMax >= 128 + 32, "a piece of a row fits");
 constexpr int kBeamFinishSmemMax = beam_finish_smem(kBeamMax, kBeamMax, kBeamFinishWarps, kBeamMax * 32 * 4);
 
 int init_device(int dev) {
@@ -287,23 +288,13 @@ int init_device(int dev) {
     SET(gru_gates_kernel, 0);
     SET(gru_finalize_kernel, 0);
     SET(wait_selftest_kernel, 0);
-    SET_SHARED((beam_scan_kernel<float, false, false>), 0);
-    SET_SHARED((beam_scan_kernel<float, false, true>), kBeamScanSmemMax);
-    SET_SHARED((beam_scan_kernel<float, true, false>), 0);
-    SET_SHARED((beam_scan_kernel<float, true, true>), kBeamScanSmemMax);
-    SET_SHARED((beam_scan_kernel<__nv_bfloat16, false, false>), 0);
-    SET_SHARED((beam_scan_kernel<__nv_bfloat16, false, true>), kBeamScanSmemMax);
-    SET_SHARED((beam_scan_kernel<__nv_bfloat16, true, false>), 0);
-    SET_SHARED((beam_scan_kernel<__nv_bfloat16, true, true>), kBeamScanSmemMax);
-    SET_SHARED((beam_finish_kernel<float, false, false>), kBeamFinishSmemMax);
-    SET_SHARED((beam_finish_kernel<float, false, true>), kBeamFinishSmemMax);
-    SET_SHARED((beam_finish_kernel<float, true, false>), kBeamFinishSmemMax);
-    SET_SHARED((beam_finish_kernel<float, true, true>), kBeamFinishSmemMax);
-    SET_SHARED((beam_finish_kernel<__nv_bfloat16, false, false>), kBeamFinishSmemMax);
-    SET_SHARED((beam_finish_kernel<__nv_bfloat16, false, true>), kBeamFinishSmemMax);
-    SET_SHARED((beam_finish_kernel<__nv_bfloat16, true, false>), kBeamFinishSmemMax);
-    SET_SHARED((beam_finish_kernel<__nv_bfloat16, true, true>), kBeamFinishSmemMax);
-    SET(beam_reorder_kernel, 0);
+    SET_SHARED(beam_reorder_kernel, 0);
+    for (int i = 0; i < 8; ++i) {
+      const bool bf16 = (i & 4) != 0, mix = (i & 2) != 0, vec = (i & 1) != 0;
+      SET_SHARED(beam_scan_kernel_for(bf16, mix, vec), vec ? kBeamScanSmemMax : 0);
+      SET_SHARED(beam_finish_kernel_for(bf16, mix, vec), kBeamFinishSmemMax);
+      SET(quantize_rows_kernel_for(bf16, vec), 0);
+    }
     SET((i8_gemm_kernel<16, __nv_bfloat16>), I8Config<16>::kSmemBytes);
     SET((i8_gemm_kernel<32, __nv_bfloat16>), I8Config<32>::kSmemBytes);
     SET((i8_gemm_kernel<64, __nv_bfloat16>), I8Config<64>::kSmemBytes);
@@ -314,10 +305,6 @@ int init_device(int dev) {
     SET((i8_gemm_kernel<64, float>), I8Config<64>::kSmemBytes);
     SET((i8_gemm_kernel<128, float>), I8Config<128>::kSmemBytes);
     SET((i8_gemm_kernel<256, float>), I8Config<256>::kSmemBytes);
-    SET((quantize_rows_kernel<float, false>), 0);
-    SET((quantize_rows_kernel<float, true>), 0);
-    SET((quantize_rows_kernel<__nv_bfloat16, false>), 0);
-    SET((quantize_rows_kernel<__nv_bfloat16, true>), 0);
 #undef SET
 #undef SET_SHARED
   }
@@ -764,13 +751,13 @@ size_t beam_plan(int n_seq, int beams, int V, int elem, bool mix, int sm_count, 
   return part0 + align256(rows * parts * sizeof(float2));
 }
 
-template <typename T, bool MIX>
-int launch_beam_select(BeamSelectArgs a, bool vec, cudaStream_t st) {
-  a.slot_bytes = beam_slot_bytes(a.scan_rows, sizeof(T), MIX);
+int launch_beam_select(BeamSelectArgs a, bool bf16, bool mix, bool vec, cudaStream_t st) {
+  const int elem = bf16 ? 2 : 4;
+  a.slot_bytes = beam_slot_bytes(a.scan_rows, elem, mix);
   DELS_CHECK_PDL("beam_scan_kernel launch",
-                 launch_pdl(vec ? beam_scan_kernel<T, MIX, true> : beam_scan_kernel<T, MIX, false>,
-                            dim3((unsigned)a.scan_ctas), dim3(32 * scan_pairs(a.scan_rows) * scan_teams(a.scan_rows)),
-                            vec ? beam_scan_smem(a.scan_rows, sizeof(T), MIX) : 0, st, a));
+                 launch_pdl(beam_scan_kernel_for(bf16, mix, vec), dim3((unsigned)a.scan_ctas),
+                            dim3(32 * scan_pairs(a.scan_rows) * scan_teams(a.scan_rows)),
+                            vec ? beam_scan_smem(a.scan_rows, elem, mix) : 0, st, a));
   // Sixteen warps or nearly: several share a beam's groups where there are few beams.  The bound
   // needs some more maxima than candidates: a lane offers its four quarters' where its
   // largest alone would be too few.
@@ -780,8 +767,7 @@ int launch_beam_select(BeamSelectArgs a, bool vec, cudaStream_t st) {
   a.finish_values = a.beams * lanes < 4 * a.select ? 4 : 1;
   const int warps = split * (a.beams < kBeamFinishWarps ? a.beams : kBeamFinishWarps);
   DELS_CHECK_PDL("beam_finish_kernel launch",
-                 launch_pdl(vec ? beam_finish_kernel<T, MIX, true> : beam_finish_kernel<T, MIX, false>,
-                            dim3((unsigned)a.n_seq), dim3(32 * warps),
+                 launch_pdl(beam_finish_kernel_for(bf16, mix, vec), dim3((unsigned)a.n_seq), dim3(32 * warps),
                             beam_finish_smem(a.beams, a.select, warps, a.beams * split * 32 * a.finish_values), st, a));
   return DELS_OK;
 }
@@ -831,17 +817,9 @@ int launch_quantize_rows(const void* x, int dtype, long long ld_x, int rows, int
                          float* scale, int sm_count, cudaStream_t st) {
   const int grid = rows < 8 * sm_count ? rows : 8 * sm_count;
   const bool vec = aligned16(x) && (ld_x * (dtype == DELS_DTYPE_BF16 ? 2 : 4)) % 16 == 0;
-  if (dtype == DELS_DTYPE_BF16) {
-    const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(x);
-    DELS_CHECK_PDL("quantize_rows_kernel launch",
-                   launch_pdl(vec ? quantize_rows_kernel<__nv_bfloat16, true> : quantize_rows_kernel<__nv_bfloat16, false>,
-                              dim3(grid), dim3(kQuantThreads), 0, st, p, ld_x, rows, K, q, ld_q, scale));
-  } else {
-    const float* p = static_cast<const float*>(x);
-    DELS_CHECK_PDL("quantize_rows_kernel launch",
-                   launch_pdl(vec ? quantize_rows_kernel<float, true> : quantize_rows_kernel<float, false>, dim3(grid),
-                              dim3(kQuantThreads), 0, st, p, ld_x, rows, K, q, ld_q, scale));
-  }
+  DELS_CHECK_PDL("quantize_rows_kernel launch",
+                 launch_pdl(quantize_rows_kernel_for(dtype == DELS_DTYPE_BF16, vec), dim3(grid), dim3(kQuantThreads), 0,
+                            st, x, ld_x, rows, K, q, ld_q, scale));
   return DELS_OK;
 }
 
@@ -1651,11 +1629,7 @@ int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const voi
   const bool mix = base != nullptr || prior != nullptr;
   beam_plan(n_seq, beams, V, (int)elem, mix, ds->sm_count < kMaxSmCount ? ds->sm_count : kMaxSmCount,
             static_cast<char*>(ws) + DELS_WS_HEADER_BYTES, &a);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == DELS_DTYPE_BF16 ? (mix ? launch_beam_select<__nv_bfloat16, true>(a, vec, st)
-                                         : launch_beam_select<__nv_bfloat16, false>(a, vec, st))
-                                  : (mix ? launch_beam_select<float, true>(a, vec, st)
-                                         : launch_beam_select<float, false>(a, vec, st));
+  return launch_beam_select(a, dtype == DELS_DTYPE_BF16, mix, vec, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t* parents, int n_seq, int beams,
@@ -1672,7 +1646,7 @@ int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t
   if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
   if (n_seq == 0) return DELS_OK;
   // the widest piece of a row that all beams' copies of it leave room for in shared memory
-  const int room = kBeamReorderSmem / beams / 16 * 16;
+  const int room = (kBeamReorderSmem / beams - 32) / 128 * 128;
   for (int first = 0; first < n_states; first += kBeamStatesPerLaunch) {
     BeamReorderArgs a;
     std::memset(&a, 0, sizeof(a));
@@ -1688,11 +1662,7 @@ int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t
       s.dst_outer = d.outer > 1 ? d.dst_outer_stride : 0;
       s.outer = (int)d.outer;
       s.inner = d.inner_bytes;
-      const unsigned long long bits = reinterpret_cast<uintptr_t>(d.src) | reinterpret_cast<uintptr_t>(d.dst) |
-                                      (unsigned long long)(s.src_row | s.dst_row | s.src_outer | s.dst_outer | s.inner);
-      s.width = 16;
-      while (s.width > 1 && bits % s.width != 0) s.width /= 2;
-      s.chunk = (int)(s.inner < room ? (s.inner + 15) / 16 * 16 : room);
+      s.chunk = (int)(s.inner < room ? s.inner : room);
       s.chunks = cdiv(s.inner, s.chunk);
       s.tile0 = a.tiles;
       a.tiles += (long long)n_seq * s.outer * s.chunks;
@@ -1703,7 +1673,7 @@ int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t
     a.beams = beams;
     a.select = select;
     a.status = status;
-    const long long most = 16ll * ds->sm_count;
+    const long long most = (long long)kBeamReorderCtas * ds->sm_count;
     DELS_CHECK_PDL("beam_reorder_kernel launch", launch_pdl(beam_reorder_kernel,
         dim3((unsigned)(a.tiles < most ? a.tiles : most)), dim3(kBeamThreads), 0,
         reinterpret_cast<cudaStream_t>(stream), a));

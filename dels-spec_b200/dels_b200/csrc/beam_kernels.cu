@@ -215,7 +215,7 @@ __device__ __forceinline__ void fold_group(const float2 (&x)[N][kPer / 2], float
 // shared memory ahead of its arithmetic (bulk copies: no registers held, a handful of
 // instructions a group).
 template <typename T, bool MIX, bool VEC>
-__global__ void __launch_bounds__(32 * kBeamScanWarps, MIX ? 5 : 8) beam_scan_kernel(const BeamSelectArgs a) {
+__global__ void __launch_bounds__(32 * kBeamScanWarps, MIX ? 5 : 8) beam_scan_kernel(BeamSelectArgs a) {
   constexpr int D = beam_scan_depth(sizeof(T), MIX);
   constexpr int N = MIX ? 2 : 1;  // rows of a warp
   extern __shared__ __align__(16) char smem[];
@@ -728,7 +728,7 @@ __device__ __noinline__ void finish_exact(const BeamSelectArgs& a, const FinishS
 // Where the bound says little (masked rows, many equal scores, more candidates than the list
 // holds) the CTA counts exactly, beam by beam.
 template <typename T, bool MIX, bool VEC>
-__global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(const BeamSelectArgs a) {
+__global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(BeamSelectArgs a) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int n_found, n_quarters;
   __shared__ uint32_t bound_key;
@@ -918,45 +918,77 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(cons
   }
 }
 
-#define DELS_BEAM_KERNELS(T, MIX, VEC)                                    \
-  template __global__ void beam_scan_kernel<T, MIX, VEC>(const BeamSelectArgs); \
-  template __global__ void beam_finish_kernel<T, MIX, VEC>(const BeamSelectArgs);
-DELS_BEAM_KERNELS(float, false, false)
-DELS_BEAM_KERNELS(float, false, true)
-DELS_BEAM_KERNELS(float, true, false)
-DELS_BEAM_KERNELS(float, true, true)
-DELS_BEAM_KERNELS(__nv_bfloat16, false, false)
-DELS_BEAM_KERNELS(__nv_bfloat16, false, true)
-DELS_BEAM_KERNELS(__nv_bfloat16, true, false)
-DELS_BEAM_KERNELS(__nv_bfloat16, true, true)
-#undef DELS_BEAM_KERNELS
+BeamKernel beam_scan_kernel_for(bool bf16, bool mix, bool vec) {
+  static const BeamKernel kernels[8] = {
+      beam_scan_kernel<float, false, false>,         beam_scan_kernel<float, false, true>,
+      beam_scan_kernel<float, true, false>,          beam_scan_kernel<float, true, true>,
+      beam_scan_kernel<__nv_bfloat16, false, false>, beam_scan_kernel<__nv_bfloat16, false, true>,
+      beam_scan_kernel<__nv_bfloat16, true, false>,  beam_scan_kernel<__nv_bfloat16, true, true>};
+  return kernels[4 * bf16 + 2 * mix + vec];
+}
+
+BeamKernel beam_finish_kernel_for(bool bf16, bool mix, bool vec) {
+  static const BeamKernel kernels[8] = {
+      beam_finish_kernel<float, false, false>,         beam_finish_kernel<float, false, true>,
+      beam_finish_kernel<float, true, false>,          beam_finish_kernel<float, true, true>,
+      beam_finish_kernel<__nv_bfloat16, false, false>, beam_finish_kernel<__nv_bfloat16, false, true>,
+      beam_finish_kernel<__nv_bfloat16, true, false>,  beam_finish_kernel<__nv_bfloat16, true, true>};
+  return kernels[4 * bf16 + 2 * mix + vec];
+}
 
 // --------------------------------------------------------------------------------
 // Reordering.  dst[b, j] = src[b, parents[b, j]] for every state.  A tile is one piece of
 // `chunk` bytes of all beams of one sequence: the rows that some child reads are staged in
 // shared memory, then every child's piece is written from there, so each byte is read once
 // however many children share a parent, and in place needs no second buffer.
+//
+// Bytes move 16 at a time whatever the alignment: a row is staged at its address modulo 16,
+// and what is written to an aligned address is put together from five 32-bit words where
+// source and destination differ modulo 16.  Bound by memory: 617 MB of a cache in place.
 // --------------------------------------------------------------------------------
 namespace {
 
-template <typename W>
-__device__ __forceinline__ void reorder_tile(const BeamState& st, const char* src, char* dst, int bytes, int beams,
-                                             int select, unsigned long long used, const int* parent, bool in_place,
-                                             char* stage) {
-  const int words = bytes / (int)sizeof(W);
-  for (int r = 0; r < beams; ++r) {
-    if (!((used >> r) & 1ull)) continue;
-    const W* s = reinterpret_cast<const W*>(src + r * st.src_row);
-    W* d = reinterpret_cast<W*>(stage + r * st.chunk);
-    for (int i = threadIdx.x; i < words; i += blockDim.x) d[i] = s[i];
+// Starts the copy of `bytes` from src to stage + src % 16 (stage 16-byte aligned), by a warp
+// that takes every `parts`-th run of 32 words.
+__device__ __forceinline__ void stage_row(char* stage, const char* src, int bytes, int part, int parts, int lane) {
+  const int shift = (int)(reinterpret_cast<uintptr_t>(src) & 15);
+  char* dst = stage + shift;
+  const int head = min(bytes, (16 - shift) & 15), words = (bytes - head) / 16, tail = bytes - head - 16 * words;
+  const uint32_t d = smem_u32(dst + head);
+  for (int i = part * 32 + lane; i < words; i += 32 * parts) cp_async_16(d + 16 * i, src + head + 16 * i, 16);
+  if (part == 0) {
+    if (lane < head) dst[lane] = src[lane];
+    if (lane < tail) dst[bytes - tail + lane] = src[bytes - tail + lane];
   }
-  __syncthreads();
-  for (int j = 0; j < select; ++j) {
-    const int p = parent[j];
-    if (p < 0 || (in_place && p == j)) continue;
-    const W* s = reinterpret_cast<const W*>(stage + p * st.chunk);
-    W* d = reinterpret_cast<W*>(dst + j * st.dst_row);
-    for (int i = threadIdx.x; i < words; i += blockDim.x) d[i] = s[i];
+}
+
+// Writes `bytes` from `from` in shared memory (any alignment) to dst, likewise.
+__device__ __forceinline__ void write_row(char* dst, const char* from, int bytes, int part, int parts, int lane) {
+  const int head = min(bytes, (int)(16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15);
+  const int words = (bytes - head) / 16, tail = bytes - head - 16 * words;
+  const char* p = from + head;
+  uint4* out = reinterpret_cast<uint4*>(dst + head);
+  const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+  if (off == 0) {
+    const uint4* in = reinterpret_cast<const uint4*>(p);
+#pragma unroll 4
+    for (int i = part * 32 + lane; i < words; i += 32 * parts) out[i] = in[i];
+  } else {
+    const uint32_t* in = reinterpret_cast<const uint32_t*>(p - (off & 3));
+    const int bits = (off & 3) * 8;
+#pragma unroll 2
+    for (int i = part * 32 + lane; i < words; i += 32 * parts) {
+      uint32_t w[5];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = in[4 * i + j];
+      w[4] = bits != 0 ? in[4 * i + 4] : 0u;
+      out[i] = make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                          __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+    }
+  }
+  if (part == 0) {
+    if (lane < head) dst[lane] = from[lane];
+    if (lane < tail) dst[bytes - tail + lane] = from[bytes - tail + lane];
   }
 }
 
@@ -966,6 +998,9 @@ __global__ void __launch_bounds__(kBeamThreads) beam_reorder_kernel(const __grid
   __shared__ __align__(16) char stage[kBeamReorderSmem];
   __shared__ int parent[kBeamMax];
   __shared__ unsigned long long used;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kWarps = kBeamThreads / 32;
+  const int row_room = kBeamReorderSmem / a.beams & ~15;
   pdl_wait();
   for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     int k = 0;
@@ -995,12 +1030,23 @@ __global__ void __launch_bounds__(kBeamThreads) beam_reorder_kernel(const __grid
     const int bytes = (int)min((long long)st.chunk, st.inner - at);
     const char* src = st.src + (long long)seq * a.beams * st.src_row + o * st.src_outer + at;
     char* dst = st.dst + (long long)seq * a.select * st.dst_row + o * st.dst_outer + at;
-    switch (st.width) {
-      case 16: reorder_tile<uint4>(st, src, dst, bytes, a.beams, a.select, used, parent, in_place, stage); break;
-      case 8: reorder_tile<uint2>(st, src, dst, bytes, a.beams, a.select, used, parent, in_place, stage); break;
-      case 4: reorder_tile<uint32_t>(st, src, dst, bytes, a.beams, a.select, used, parent, in_place, stage); break;
-      case 2: reorder_tile<uint16_t>(st, src, dst, bytes, a.beams, a.select, used, parent, in_place, stage); break;
-      default: reorder_tile<uint8_t>(st, src, dst, bytes, a.beams, a.select, used, parent, in_place, stage); break;
+    // a warp per row, or several where there are few
+    const unsigned long long rows = used;
+    int parts = a.beams < kWarps ? kWarps / a.beams : 1;
+    for (int i = warp; i < a.beams * parts; i += kWarps) {
+      const int r = i / parts;
+      if ((rows >> r) & 1ull) stage_row(stage + r * row_room, src + r * st.src_row, bytes, i % parts, parts, lane);
+    }
+    cp_async_commit();
+    cp_async_wait_all();
+    __syncthreads();
+    parts = a.select < kWarps ? kWarps / a.select : 1;
+    for (int i = warp; i < a.select * parts; i += kWarps) {
+      const int j = i / parts, p = parent[j];
+      if (p < 0 || (in_place && p == j)) continue;
+      const char* s = src + p * st.src_row;
+      write_row(dst + j * st.dst_row, stage + p * row_room + (reinterpret_cast<uintptr_t>(s) & 15), bytes, i % parts,
+                parts, lane);
     }
   }
 }

@@ -88,10 +88,11 @@ constexpr int beam_finish_smem(int beams, int select, int warps, int values) {
   return (beams * 8 + 15) / 16 * 16 + (listing > exact ? listing : exact);
 }
 
-template <typename T, bool MIX, bool VEC>
-__global__ void beam_scan_kernel(const BeamSelectArgs a);
-template <typename T, bool MIX, bool VEC>
-__global__ void beam_finish_kernel(const BeamSelectArgs a);
+// The kernels for bf16 or fp32 logits, with shared terms (mix) or without, and with 16-byte
+// loads (vec) or without.
+using BeamKernel = void (*)(BeamSelectArgs);
+BeamKernel beam_scan_kernel_for(bool bf16, bool mix, bool vec);
+BeamKernel beam_finish_kernel_for(bool bf16, bool mix, bool vec);
 
 // One state of the beams: rows x outer x inner contiguous bytes.
 struct BeamState {
@@ -101,7 +102,6 @@ struct BeamState {
   long long inner;                                   // bytes
   int outer;
   int chunk;         // bytes of one tile's piece of `inner`
-  int width;         // bytes moved at once: 16, 8, 4, 2 or 1
   int chunks;        // pieces of `inner`
   long long tile0;   // first tile of this state
 };
@@ -118,7 +118,9 @@ struct BeamReorderArgs {
   long long tiles;
 };
 
-constexpr int kBeamReorderSmem = 32768;
+// A tile's stage: each beam's piece, up to 15 bytes before it and a word after.
+constexpr int kBeamReorderSmem = 33792;
+constexpr int kBeamReorderCtas = 5;  // an SM holds: 617 MB of a cache in 97 us; a sixth would wait its turn (126 us)
 
 __global__ void beam_reorder_kernel(const __grid_constant__ BeamReorderArgs a);
 

@@ -326,8 +326,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 // Rows to 8 bits (i8_kernels.cu): scale = max |x| / 127, q = rint(x * (127 / max |x|)).
 constexpr int kQuantThreads = 256;
-template <typename T, bool VEC>
-__global__ void quantize_rows_kernel(const T* x, long long ld_x, int rows, int K, int8_t* q, long long ld_q,
-                                     float* scale);
+using QuantizeKernel = void (*)(const void* x, long long ld_x, int rows, int K, int8_t* q, long long ld_q, float* scale);
+// for bf16 or fp32 rows, with 16-byte loads (vec) or without
+QuantizeKernel quantize_rows_kernel_for(bool bf16, bool vec);
 
 }  // namespace dels

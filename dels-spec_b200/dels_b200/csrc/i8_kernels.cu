@@ -33,14 +33,14 @@ __device__ __forceinline__ int to_i8(float x, float inv) {
 }  // namespace
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* x, long long ld_x, int rows, int K,
+__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const void* x, long long ld_x, int rows, int K,
                                                                       int8_t* q, long long ld_q, float* scale) {
   __shared__ float warp_top[kQuantThreads / 32];
   const int t = threadIdx.x;
   pdl_wait();
   pdl_trigger();
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* src = x + (long long)row * ld_x;
+    const T* src = static_cast<const T*>(x) + (long long)row * ld_x;
     int8_t* dst = q + (long long)row * ld_q;
     const int whole = VEC ? K / 8 * 8 : 0;
     float top = 0.0f;
@@ -78,13 +78,9 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* x
   }
 }
 
-template __global__ void quantize_rows_kernel<float, true>(const float*, long long, int, int, int8_t*, long long,
-                                                           float*);
-template __global__ void quantize_rows_kernel<float, false>(const float*, long long, int, int, int8_t*, long long,
-                                                            float*);
-template __global__ void quantize_rows_kernel<__nv_bfloat16, true>(const __nv_bfloat16*, long long, int, int, int8_t*,
-                                                                   long long, float*);
-template __global__ void quantize_rows_kernel<__nv_bfloat16, false>(const __nv_bfloat16*, long long, int, int, int8_t*,
-                                                                    long long, float*);
+QuantizeKernel quantize_rows_kernel_for(bool bf16, bool vec) {
+  if (bf16) return vec ? quantize_rows_kernel<__nv_bfloat16, true> : quantize_rows_kernel<__nv_bfloat16, false>;
+  return vec ? quantize_rows_kernel<float, true> : quantize_rows_kernel<float, false>;
+}
 
 }  // namespace dels
