@@ -202,7 +202,7 @@ int make_map_vec_f32(CUtensorMap* m, const float* ptr, long long n, int box_n) {
 struct DeviceState {
   bool ready = false;
   int sm_count = 0;
-  int max_pairs = 0;  // co-resident 2-CTA clusters of the paired scorer
+  int max_pairs = 0;  // co-resident 2-CTA clusters of the paired kernels (one CTA an SM)
 };
 DeviceState g_dev[kMaxDevices];
 std::mutex g_dev_mu;
@@ -300,6 +300,8 @@ int init_device(int dev) {
     SET((i8_gemm_kernel<64, __nv_bfloat16>), I8Config<64>::kSmemBytes);
     SET((i8_gemm_kernel<128, __nv_bfloat16>), I8Config<128>::kSmemBytes);
     SET((i8_gemm_kernel<256, __nv_bfloat16>), I8Config<256>::kSmemBytes);
+    SET(i8_pair_kernel<__nv_bfloat16>, I8PairConfig::kSmemBytes);
+    SET(i8_pair_kernel<float>, I8PairConfig::kSmemBytes);
     SET((i8_gemm_kernel<16, float>), I8Config<16>::kSmemBytes);
     SET((i8_gemm_kernel<32, float>), I8Config<32>::kSmemBytes);
     SET((i8_gemm_kernel<64, float>), I8Config<64>::kSmemBytes);
@@ -854,8 +856,32 @@ int launch_i8_tn(const void* xq, long long ld_x, const void* wq, long long ld_w,
 }
 
 template <typename OutT>
+int launch_i8_pair(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, I8Args a, int max_pairs,
+                   cudaStream_t st) {
+  int rc = ensure_encode();
+  if (rc != DELS_OK) return rc;
+  using Cfg = I8PairConfig;
+  a.m_tiles = cdiv(a.rows, Cfg::BN);
+  a.n_tiles = cdiv(a.n_out, 2 * kBM);
+  a.kb = cdiv(K, kI8BK);
+  a.tail = kScorerTailSplit;
+  const long long tiles = (long long)a.m_tiles * a.n_tiles;
+  const long long want = tiles < max_pairs ? tiles * a.tail : tiles;
+  CUtensorMap mw, mx, mxt;
+  if ((rc = make_map_i8(&mw, wq, K, a.n_out, ld_w, kBM)) != DELS_OK) return rc;
+  if ((rc = make_map_i8(&mx, xq, K, a.rows, ld_x, Cfg::BN / 2)) != DELS_OK) return rc;
+  if ((rc = make_map_i8(&mxt, xq, K, a.rows, ld_x, Cfg::BN / 2 / a.tail)) != DELS_OK) return rc;
+  DELS_CHECK_PDL("i8_pair_kernel launch",
+                 launch_pdl(i8_pair_kernel<OutT>, dim3((unsigned)(2 * (want < max_pairs ? want : max_pairs))),
+                            dim3(kTcThreads), Cfg::kSmemBytes, st, mw, mx, mxt, a));
+  return DELS_OK;
+}
+
+template <typename OutT>
 int launch_i8_out(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, const I8Args& a, int sm_count,
-                  cudaStream_t st) {
+                  int max_pairs, cudaStream_t st) {
+  if (a.rows > kBM && max_pairs > 0 && g_use_pairs)
+    return launch_i8_pair<OutT>(xq, ld_x, wq, ld_w, K, a, max_pairs, st);
   if (a.rows <= 16) return launch_i8_tn<16, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
   if (a.rows <= 32) return launch_i8_tn<32, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
   if (a.rows <= 64) return launch_i8_tn<64, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
@@ -875,7 +901,7 @@ int check_i8_out(const void* out, int out_dtype, long long ld_out, const void* b
 
 int launch_i8(const void* xq, long long ld_x, const float* x_scale, const void* wq, long long ld_w,
               const float* w_scale, const void* bias, int rows, int K, int N, void* out, int out_dtype,
-              long long ld_out, bool early, int* status, int sm_count, cudaStream_t st) {
+              long long ld_out, bool early, int* status, const DeviceState& ds, cudaStream_t st) {
   I8Args a;
   std::memset(&a, 0, sizeof(a));
   a.rows = rows;
@@ -888,8 +914,8 @@ int launch_i8(const void* xq, long long ld_x, const float* x_scale, const void* 
   a.store2 = N % 2 == 0 && ld_out % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
   a.early = early && g_use_pdl;
   a.status = status;
-  return out_dtype == DELS_DTYPE_BF16 ? launch_i8_out<__nv_bfloat16>(xq, ld_x, wq, ld_w, K, a, sm_count, st)
-                                      : launch_i8_out<float>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
+  return out_dtype == DELS_DTYPE_BF16 ? launch_i8_out<__nv_bfloat16>(xq, ld_x, wq, ld_w, K, a, ds.sm_count, ds.max_pairs, st)
+                                      : launch_i8_out<float>(xq, ld_x, wq, ld_w, K, a, ds.sm_count, ds.max_pairs, st);
 }
 
 // Row stride of the quantised rows that a fused call keeps in its workspace.
@@ -1717,7 +1743,7 @@ int dels_linear_i8(const int8_t* xq, int64_t ld_xq, const float* x_scale, const 
   if (rows == 0) return DELS_OK;
   // the kernel before this one may be the one that quantised the weights
   return launch_i8(xq, ld_xq, x_scale, wq, ld_wq, w_scale, bias, rows, K, N, out, out_dtype, ld_out, false, hdr.status,
-                   ds->sm_count, reinterpret_cast<cudaStream_t>(stream));
+                   *ds, reinterpret_cast<cudaStream_t>(stream));
 }
 
 size_t dels_linear_w8a8_workspace_bytes(int rows, int K) {
@@ -1743,7 +1769,7 @@ int dels_linear_w8a8(const void* x, int x_dtype, int64_t ld_x, const int8_t* wq,
   if ((rc = dels_quantize_rows_i8(x, x_dtype, ld_x, rows, K, xq, i8_padded(K), x_scale, stream)) != DELS_OK) return rc;
   if (rows == 0) return DELS_OK;
   return launch_i8(xq, i8_padded(K), x_scale, wq, ld_wq, w_scale, bias, rows, K, N, out, out_dtype, ld_out, true,
-                   hdr.status, ds->sm_count, reinterpret_cast<cudaStream_t>(stream));
+                   hdr.status, *ds, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -12,7 +12,8 @@
 // in a ring; two accumulators in TMEM let a tile's epilogue overlap the next one's MMAs.
 //
 // Warp roles (192 threads): warp 0 = TMA producer, warp 1 = TMEM allocator + MMA issuer,
-// warps 2..5 = epilogue (one thread per channel).
+// warps 2..5 = epilogue (one thread per channel).  Above 128 rows CTA pairs share the tiles
+// (i8_pair_kernel).
 #pragma once
 
 #include "tc_gemm.cuh"
@@ -31,6 +32,7 @@ struct I8Args {
   void* out;               // [rows, n_out] bf16 or fp32
   long long ld_out;
   int store2;              // bf16: two channels per store (even ld_out, 4-byte aligned out)
+  int tail;                // i8_pair_kernel: ways a tile of the last wave is split along the rows
   int early;               // the weights are not written by the previous kernel: load them before waiting for it
   int* status;
 };
@@ -321,6 +323,276 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, Cfg::kTmemCols);
+  }
+}
+
+// --------------------------------------------------------------------------------
+// The same product on CTA pairs (tcgen05.mma.cta_group::2), for more than 128 rows: a tile is
+// 256 channels x 256 rows, each CTA stages its 128 channels and half of the rows' tile, so a
+// block of K moves 32 KB through each SM's shared memory for the work that takes 48 KB in
+// i8_gemm_kernel.  The barriers are those of tc_scorer_pair_kernel: rank 0 issues the MMAs of
+// both CTAs, whose copies complete on rank 0's full barriers.  Two blocks of K form a stage
+// (256 contiguous bytes of every channel).  The last, partial wave's tiles are split along the
+// rows (make_schedule's tail).
+// --------------------------------------------------------------------------------
+struct I8PairConfig {
+  static constexpr int BN = 256;                 // rows of a tile
+  static constexpr int kGroup = 2;               // blocks of K in a stage
+  static constexpr int kABytes = kBM * kI8BK;
+  static constexpr int kBBytes = BN / 2 * kI8BK;
+  static constexpr int kSlots = 6;
+  static constexpr int kStages = kSlots / kGroup;
+  static constexpr int kScaleOffset = kSlots * (kABytes + kBBytes);  // [4 warps][BN] row scales
+  static constexpr int kBarOffset = kScaleOffset + 4 * BN * 4;
+  static constexpr int kNumBars = 2 * kStages + 4;
+  static constexpr int kSmemBytes = kBarOffset + kNumBars * 8 + 16 + 1024;
+  static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
+__device__ __forceinline__ void tc_mma_pair_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// map_x / map_xt: the rows in boxes of 128 and of 128 / args.tail (a split tile's half).
+template <typename OutT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
+    i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                   const __grid_constant__ CUtensorMap map_xt, const I8Args args) {
+  using Cfg = I8PairConfig;
+  constexpr int S = Cfg::kStages, KG = Cfg::kGroup, BN = Cfg::BN;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base_addr = (raw_addr + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base_addr - raw_addr);
+  const uint32_t a_base = base_addr;
+  const uint32_t b_base = base_addr + Cfg::kSlots * Cfg::kABytes;
+  float* scales = reinterpret_cast<float*>(smem + Cfg::kScaleOffset);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  auto full_bar = [&](int s) { return smem_u32(&bars[s]); };
+  auto empty_bar = [&](int s) { return smem_u32(&bars[S + s]); };
+  auto tfull_bar = [&](int a) { return smem_u32(&bars[2 * S + a]); };
+  auto tempty_bar = [&](int a) { return smem_u32(&bars[2 * S + 2 + a]); };
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), 8);  // 4 epilogue warps in each CTA
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_map(&map_w);
+    tma_prefetch_map(&map_x);
+    tma_prefetch_map(&map_xt);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers are initialised
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();
+  // "columns" of the schedule are row tiles, its "row tiles" the weight tiles of this product:
+  // neighbouring units share a weight tile
+  const Schedule sched = make_schedule(args.m_tiles, args.n_tiles, 1, args.m_tiles, args.tail, num_pairs);
+  // a unit: weight tile, first row, rows (BN or a split tile's)
+  auto unit = [&](int u, int& n_tile, int& m0, int& rows, bool& tail) {
+    tail = u >= sched.main_units;
+    const int q = u - sched.main_units;
+    const int t = tail ? sched.main_units + q / sched.tail_split : u;
+    n_tile = t / args.m_tiles;
+    rows = tail ? BN / sched.tail_split : BN;
+    m0 = t % args.m_tiles * BN + (tail ? q % sched.tail_split * rows : 0);
+  };
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer (both CTAs)
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = pair; u < sched.total_units && ok; u += num_pairs) {
+        int n_tile, m0, rows;
+        bool tail;
+        unit(u, n_tile, m0, rows, tail);
+        const int n0 = n_tile * 2 * kBM + (int)rank * kBM, x0 = m0 + (int)rank * (rows / 2);
+        const CUtensorMap* mx = tail ? &map_xt : &map_x;
+        const uint32_t tx_pair = 2u * ((uint32_t)Cfg::kABytes + (uint32_t)(rows / 2) * kI8BK);
+        for (int kb = 0; kb < args.kb; kb += KG) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, args.status)) {
+            ok = false;
+            break;
+          }
+          const int nb = args.kb - kb < KG ? args.kb - kb : KG;
+          const uint32_t full_leader = mapa_shared(full_bar(stage), 0);
+          if (leader) mbar_arrive_expect_tx(full_bar(stage), tx_pair * (uint32_t)nb);
+          for (int j = 0; j < nb; ++j) {
+            const int slot = stage * KG + j, k = (kb + j) * kI8BK;
+            tma_load_2d_pair(a_base + slot * Cfg::kABytes, &map_w, full_leader, k, n0);
+            tma_load_2d_pair(b_base + slot * Cfg::kBBytes, mx, full_leader, k, x0);
+          }
+          ++issued;
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        // Aborting: the copies in flight complete on rank 0's full barriers; rank 0 drains
+        // them, the peer waits out the same bounded delay before leaving.
+        const unsigned long long t0 = globaltimer_ns();
+        const int outstanding = issued < S ? issued : S;
+        for (int i = 0; i < outstanding && leader; ++i) {
+          if (--stage < 0) {
+            stage = S - 1;
+            phase ^= 1u;
+          }
+          while (!mbar_try_wait(full_bar(stage), phase) && globaltimer_ns() - t0 < kWaitLimitNs / 20) {
+          }
+        }
+        while (!leader && globaltimer_ns() - t0 < kWaitLimitNs / 40) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer (rank 0)
+    if (lane == 0 && leader) {
+      constexpr uint32_t idesc_full = make_idesc_s8_s32(2 * kBM, BN);
+      const uint32_t idesc_tail = make_idesc_s8_s32(2 * kBM, BN / sched.tail_split);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int u = pair; u < sched.total_units && ok; u += num_pairs) {
+        const uint32_t idesc = u >= sched.main_units ? idesc_tail : idesc_full;
+        if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, args.status)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+        for (int kb = 0; kb < args.kb; kb += KG) {
+          if (!mbar_wait(full_bar(stage), phase, abort_flag, args.status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int nb = args.kb - kb < KG ? args.kb - kb : KG;
+          for (int j = 0; j < nb; ++j) {
+            const int slot = stage * KG + j;
+            const uint64_t adesc = make_sw128_desc(a_base + slot * Cfg::kABytes);
+            const uint64_t bdesc = make_sw128_desc(b_base + slot * Cfg::kBBytes);
+#pragma unroll
+            for (int k = 0; k < kI8BK / 32; ++k)
+              tc_mma_pair_i8(d_tmem, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc,
+                             (kb + j > 0 || k > 0) ? 1u : 0u);
+          }
+          tc_commit_pair_both(empty_bar(stage));
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        tc_commit_pair_both(tfull_bar(acc));
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      if (!ok || *abort_flag) {
+        const uint32_t drain = tfull_bar(acc);
+        tc_commit_pair_both(drain);
+        const unsigned long long t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, acc_phase) && globaltimer_ns() - t0 < kWaitLimitNs / 20) {
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue (both CTAs)
+    const int quad = warp & 3;
+    float* scale = scales + quad * BN;
+    const uint32_t tempty_leader0 = mapa_shared(tempty_bar(0), 0);
+    const uint32_t tempty_leader1 = mapa_shared(tempty_bar(1), 0);
+    OutT* out = static_cast<OutT*>(args.out);
+    const OutT* bias_v = static_cast<const OutT*>(args.bias);
+    int acc = 0, scale_m = -1;
+    uint32_t acc_phase = 0;
+    for (int u = pair; u < sched.total_units; u += num_pairs) {
+      int n_tile, m0, rows;
+      bool tail;
+      unit(u, n_tile, m0, rows, tail);
+      const int n = n_tile * 2 * kBM + (int)rank * kBM + quad * 32 + lane;
+      const bool channel_ok = n < args.n_out, warp_ok = n - lane < args.n_out;
+      const int valid = min(rows, args.rows - m0);  // may be <= 0 in a split tile
+      if (m0 != scale_m) {
+        __syncwarp();
+        for (int j = lane; j < rows; j += 32) scale[j] = m0 + j < args.rows ? __ldg(args.sx + m0 + j) : 0.0f;
+        __syncwarp();
+        scale_m = m0;
+      }
+      const float sw = channel_ok ? __ldg(args.sw + n) : 0.0f;
+      float bias = 0.0f;
+      if (channel_ok && bias_v != nullptr) {
+        if constexpr (sizeof(OutT) == 2)
+          bias = __bfloat162float(bias_v[n]);
+        else
+          bias = bias_v[n];
+      }
+      if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, args.status)) break;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
+      OutT* dst = out + (long long)m0 * args.ld_out + n;
+#pragma unroll 1
+      for (int c = 0; c < (warp_ok ? valid : 0); c += 32) {
+        uint32_t v[32];
+        tmem_ld_32cols(t_row + (uint32_t)c, v);
+        tmem_ld_wait(v);
+        i8_store<32, OutT>(v, scale + c, sw, bias, valid - c, channel_ok, dst + (long long)c * args.ld_out, args.ld_out,
+                           args.store2 != 0, lane);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (leader)
+          mbar_arrive(tempty_bar(acc));
+        else
+          mbar_arrive_remote(acc == 0 ? tempty_leader0 : tempty_leader1);
+      }
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the partner no longer touches this CTA's shared memory / TMEM
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
   }
 }
 
