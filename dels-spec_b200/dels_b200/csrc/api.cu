@@ -295,18 +295,20 @@ int init_device(int dev) {
       SET_SHARED(beam_finish_kernel_for(bf16, mix, vec), kBeamFinishSmemMax);
       SET(quantize_rows_kernel_for(bf16, vec), 0);
     }
-    SET((i8_gemm_kernel<16, __nv_bfloat16>), I8Config<16>::kSmemBytes);
-    SET((i8_gemm_kernel<32, __nv_bfloat16>), I8Config<32>::kSmemBytes);
-    SET((i8_gemm_kernel<64, __nv_bfloat16>), I8Config<64>::kSmemBytes);
-    SET((i8_gemm_kernel<128, __nv_bfloat16>), I8Config<128>::kSmemBytes);
-    SET((i8_gemm_kernel<256, __nv_bfloat16>), I8Config<256>::kSmemBytes);
+    for (int i = 0; i < 12; ++i)
+      SET(i8_gemv_kernel_for((I8Source)(i % 3), (i / 3 & 1) != 0, 1 << i / 6), kI8GemvBytes);
+    SET((i8_gemm_kernel<16, __nv_bfloat16>), I8Config<16>::kMaxBytes);
+    SET((i8_gemm_kernel<32, __nv_bfloat16>), I8Config<32>::kMaxBytes);
+    SET((i8_gemm_kernel<64, __nv_bfloat16>), I8Config<64>::kMaxBytes);
+    SET((i8_gemm_kernel<128, __nv_bfloat16>), I8Config<128>::kMaxBytes);
+    SET((i8_gemm_kernel<256, __nv_bfloat16>), I8Config<256>::kMaxBytes);
     SET(i8_pair_kernel<__nv_bfloat16>, I8PairConfig::kSmemBytes);
     SET(i8_pair_kernel<float>, I8PairConfig::kSmemBytes);
-    SET((i8_gemm_kernel<16, float>), I8Config<16>::kSmemBytes);
-    SET((i8_gemm_kernel<32, float>), I8Config<32>::kSmemBytes);
-    SET((i8_gemm_kernel<64, float>), I8Config<64>::kSmemBytes);
-    SET((i8_gemm_kernel<128, float>), I8Config<128>::kSmemBytes);
-    SET((i8_gemm_kernel<256, float>), I8Config<256>::kSmemBytes);
+    SET((i8_gemm_kernel<16, float>), I8Config<16>::kMaxBytes);
+    SET((i8_gemm_kernel<32, float>), I8Config<32>::kMaxBytes);
+    SET((i8_gemm_kernel<64, float>), I8Config<64>::kMaxBytes);
+    SET((i8_gemm_kernel<128, float>), I8Config<128>::kMaxBytes);
+    SET((i8_gemm_kernel<256, float>), I8Config<256>::kMaxBytes);
 #undef SET
 #undef SET_SHARED
   }
@@ -815,6 +817,16 @@ int check_i8_shape(int rows, int K, int N) {
   return DELS_OK;
 }
 
+int check_quantize(const void* x, int dtype, long long ld_x, int rows, int K) {
+  if (rows < 0 || K <= 0) return fail(DELS_ERR_INVALID_ARG, "bad shape rows=%d K=%d", rows, K);
+  if (dtype != DELS_DTYPE_BF16 && dtype != DELS_DTYPE_F32) return fail(DELS_ERR_INVALID_ARG, "unknown dtype %d", dtype);
+  if (rows > 0 && x == nullptr) return fail(DELS_ERR_INVALID_ARG, "x is NULL");
+  if (ld_x < K) return fail(DELS_ERR_INVALID_ARG, "ld_x %lld < K %d", ld_x, K);
+  if (reinterpret_cast<uintptr_t>(x) % (dtype == DELS_DTYPE_BF16 ? 2 : 4) != 0)
+    return fail(DELS_ERR_ALIGNMENT, "x must be aligned to its elements");
+  return DELS_OK;
+}
+
 int launch_quantize_rows(const void* x, int dtype, long long ld_x, int rows, int K, int8_t* q, long long ld_q,
                          float* scale, int sm_count, cudaStream_t st) {
   const int grid = rows < 8 * sm_count ? rows : 8 * sm_count;
@@ -825,33 +837,47 @@ int launch_quantize_rows(const void* x, int dtype, long long ld_x, int rows, int
   return DELS_OK;
 }
 
+// A tile shape of i8_gemm_kernel: rows of a tile and channels that a weight tile loads, and
+// what the whole product then costs: waves of tiles times a block of K's cost, in channels.  A
+// block costs its bytes (box channels, and the rows, which come from L2) and a hand-off worth
+// about 32 channels; wide tiles take at least as long as 128 lanes' MMAs, about TN / 2.
+struct I8Shape {
+  int tn, box;
+  long long cost;
+};
+
+I8Shape plan_i8(int rows, int n_out, int sm_count) {
+  I8Shape best = {0, 0, -1};
+  for (int tn = 16; tn <= 256; tn *= 2) {
+    if (tn > 16 && tn / 2 >= rows) break;
+    for (int box = 8; box <= kBM; box += 8) {
+      const long long units = (long long)cdiv(n_out, box) * cdiv(rows, tn);
+      const int block = box + tn / 2 > tn ? box + tn / 2 : tn;
+      const long long cost = cdiv(units, sm_count) * (32ll + block);
+      if (best.cost < 0 || cost <= best.cost) best = {tn, box, cost};
+    }
+  }
+  return best;
+}
+
 template <int TN, typename OutT>
-int launch_i8_tn(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, I8Args a, int sm_count,
+int launch_i8_tn(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, I8Args a, int box, int sm_count,
                  cudaStream_t st) {
   int rc = ensure_encode();
   if (rc != DELS_OK) return rc;
   a.m_tiles = cdiv(a.rows, TN);
-  // Channels a weight tile loads: the height whose waves take the shortest.  A block of K
-  // costs its bytes or its MMAs (128 lanes run however few are loaded: about as long as
-  // TN / 2 channels take to load), and a hand-off worth about 32 channels.
-  long long best = -1;
-  for (int box = 8; box <= kBM; box += 8) {
-    const long long units = (long long)cdiv(a.n_out, box) * a.m_tiles;
-    const long long cost = (long long)cdiv(units, sm_count) * (32 + (box > TN / 2 ? box : TN / 2));
-    if (best < 0 || cost <= best) {
-      best = cost;
-      a.box = box;
-    }
-  }
-  a.n_tiles = cdiv(a.n_out, a.box);
+  a.box = box;
+  a.n_tiles = cdiv(a.n_out, box);
   a.kb = cdiv(K, kI8BK);
+  a.stages = I8Config<TN>::stages(box, a.kb);
   CUtensorMap mw, mx;
   if ((rc = make_map_i8(&mw, wq, K, a.n_out, ld_w, a.box)) != DELS_OK) return rc;
   if ((rc = make_map_i8(&mx, xq, K, a.rows, ld_x, TN)) != DELS_OK) return rc;
   const long long units = (long long)a.n_tiles * a.m_tiles;
   DELS_CHECK_PDL("i8_gemm_kernel launch",
                  launch_pdl(i8_gemm_kernel<TN, OutT>, dim3((unsigned)(units < sm_count ? units : sm_count)),
-                            dim3(kTcThreads), I8Config<TN>::kSmemBytes, st, mw, mx, a));
+                            dim3(kI8Threads), I8Config<TN>::kFixedBytes + a.stages * I8Config<TN>::slot_bytes(box), st,
+                            mw, mx, a));
   return DELS_OK;
 }
 
@@ -880,13 +906,32 @@ int launch_i8_pair(const void* xq, long long ld_x, const void* wq, long long ld_
 template <typename OutT>
 int launch_i8_out(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, const I8Args& a, int sm_count,
                   int max_pairs, cudaStream_t st) {
-  if (a.rows > kBM && max_pairs > 0 && g_use_pairs)
-    return launch_i8_pair<OutT>(xq, ld_x, wq, ld_w, K, a, max_pairs, st);
-  if (a.rows <= 16) return launch_i8_tn<16, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
-  if (a.rows <= 32) return launch_i8_tn<32, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
-  if (a.rows <= 64) return launch_i8_tn<64, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
-  if (a.rows <= 128) return launch_i8_tn<128, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
-  return launch_i8_tn<256, OutT>(xq, ld_x, wq, ld_w, K, a, sm_count, st);
+  const I8Shape shape = plan_i8(a.rows, a.n_out, sm_count);
+  if (a.rows > kBM && max_pairs > 0 && g_use_pairs) {
+    // Pairs where their large tiles fill the device: a pair's block of K costs what a 256-row
+    // tile's does.
+    const long long tiles = (long long)cdiv(a.rows, I8PairConfig::BN) * cdiv(a.n_out, 2 * kBM);
+    if (cdiv(tiles, max_pairs) * (32ll + 256) <= shape.cost + shape.cost / 8)
+      return launch_i8_pair<OutT>(xq, ld_x, wq, ld_w, K, a, max_pairs, st);
+  }
+  switch (shape.tn) {
+    case 16: return launch_i8_tn<16, OutT>(xq, ld_x, wq, ld_w, K, a, shape.box, sm_count, st);
+    case 32: return launch_i8_tn<32, OutT>(xq, ld_x, wq, ld_w, K, a, shape.box, sm_count, st);
+    case 64: return launch_i8_tn<64, OutT>(xq, ld_x, wq, ld_w, K, a, shape.box, sm_count, st);
+    case 128: return launch_i8_tn<128, OutT>(xq, ld_x, wq, ld_w, K, a, shape.box, sm_count, st);
+    default: return launch_i8_tn<256, OutT>(xq, ld_x, wq, ld_w, K, a, shape.box, sm_count, st);
+  }
+}
+
+// Whether the one-launch form for a few rows takes the product.
+bool i8_few_rows(int rows, int K) { return rows <= kI8GemvRows && (long long)rows * ((K + 15) / 16 * 16) <= kI8GemvBytes; }
+
+int launch_i8_gemv(const I8GemvArgs& a, I8Source source, bool out_bf16, int sm_count, cudaStream_t st) {
+  const int most = kI8GemvCtas * sm_count, want = cdiv(a.n_out, kI8GemvThreads / 32);
+  DELS_CHECK_PDL("i8_gemv_kernel launch",
+                 launch_pdl(i8_gemv_kernel_for(source, out_bf16, a.rows), dim3(want < most ? want : most),
+                            dim3(kI8GemvThreads), (size_t)a.rows * ((a.K + 15) / 16 * 16), st, a));
+  return DELS_OK;
 }
 
 int check_i8_out(const void* out, int out_dtype, long long ld_out, const void* bias, int N) {
@@ -1710,12 +1755,8 @@ int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t
 int dels_quantize_rows_i8(const void* x, int dtype, int64_t ld_x, int rows, int K, int8_t* q, int64_t ld_q,
                           float* scale, void* stream) {
   int rc;
-  if (rows < 0 || K <= 0) return fail(DELS_ERR_INVALID_ARG, "bad shape rows=%d K=%d", rows, K);
-  if (dtype != DELS_DTYPE_BF16 && dtype != DELS_DTYPE_F32) return fail(DELS_ERR_INVALID_ARG, "unknown dtype %d", dtype);
-  if (rows > 0 && (x == nullptr || scale == nullptr)) return fail(DELS_ERR_INVALID_ARG, "NULL argument");
-  if (ld_x < K) return fail(DELS_ERR_INVALID_ARG, "ld_x %lld < K %d", (long long)ld_x, K);
-  if (reinterpret_cast<uintptr_t>(x) % (dtype == DELS_DTYPE_BF16 ? 2 : 4) != 0)
-    return fail(DELS_ERR_ALIGNMENT, "x must be aligned to its elements");
+  if ((rc = check_quantize(x, dtype, ld_x, rows, K)) != DELS_OK) return rc;
+  if (rows > 0 && scale == nullptr) return fail(DELS_ERR_INVALID_ARG, "scale is NULL");
   if (rows > 0 && (rc = check_i8_matrix("q", q, ld_q, K)) != DELS_OK) return rc;
   DeviceState* ds = nullptr;
   if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
@@ -1741,6 +1782,9 @@ int dels_linear_i8(const int8_t* xq, int64_t ld_xq, const float* x_scale, const 
   DeviceState* ds = nullptr;
   if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
   if (rows == 0) return DELS_OK;
+  if (i8_few_rows(rows, K))
+    return launch_i8_gemv({xq, ld_xq, 1, x_scale, wq, ld_wq, w_scale, bias, out, ld_out, rows, K, N}, kI8FromInt8,
+                          out_dtype == DELS_DTYPE_BF16, ds->sm_count, reinterpret_cast<cudaStream_t>(stream));
   // the kernel before this one may be the one that quantised the weights
   return launch_i8(xq, ld_xq, x_scale, wq, ld_wq, w_scale, bias, rows, K, N, out, out_dtype, ld_out, false, hdr.status,
                    *ds, reinterpret_cast<cudaStream_t>(stream));
@@ -1763,6 +1807,13 @@ int dels_linear_w8a8(const void* x, int x_dtype, int64_t ld_x, const int8_t* wq,
   if ((rc = ws_header(ws, ws_bytes, dels_linear_w8a8_workspace_bytes(rows, K), &hdr)) != DELS_OK) return rc;
   DeviceState* ds = nullptr;
   if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
+  if (rows > 0 && i8_few_rows(rows, K)) {
+    if ((rc = check_quantize(x, x_dtype, ld_x, rows, K)) != DELS_OK) return rc;
+    const bool vec = aligned16(x) && (ld_x * (x_dtype == DELS_DTYPE_BF16 ? 2 : 4)) % 16 == 0;
+    return launch_i8_gemv({x, ld_x, vec, nullptr, wq, ld_wq, w_scale, bias, out, ld_out, rows, K, N},
+                          x_dtype == DELS_DTYPE_BF16 ? kI8FromBf16 : kI8FromF32, out_dtype == DELS_DTYPE_BF16,
+                          ds->sm_count, reinterpret_cast<cudaStream_t>(stream));
+  }
   char* body = static_cast<char*>(ws) + DELS_WS_HEADER_BYTES;
   float* x_scale = reinterpret_cast<float*>(body);
   int8_t* xq = reinterpret_cast<int8_t*>(body + align256((size_t)rows * sizeof(float)));

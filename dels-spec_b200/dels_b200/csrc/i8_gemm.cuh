@@ -11,8 +11,8 @@
 // K goes in blocks of 128 (one 128-byte swizzled line of every operand row), staged by TMA
 // in a ring; two accumulators in TMEM let a tile's epilogue overlap the next one's MMAs.
 //
-// Warp roles (192 threads): warp 0 = TMA producer, warp 1 = TMEM allocator + MMA issuer,
-// warps 2..5 = epilogue (one thread per channel).  Above 128 rows CTA pairs share the tiles
+// Warp roles (224 threads): warps 0 and 6 = TMA producers (weights, rows), warp 1 = TMEM
+// allocator + MMA issuer, warps 2..5 = epilogue (one thread per channel).  Above 128 rows CTA pairs share the tiles
 // (i8_pair_kernel).
 #pragma once
 
@@ -21,10 +21,12 @@
 namespace dels {
 
 constexpr int kI8BK = 128;  // K elements (bytes) of a block
+constexpr int kI8Threads = 224;
 
 struct I8Args {
   int rows, n_out, kb;     // kb: blocks of K
   int box;                 // channels a weight tile loads (<= 128; the MMA always runs 128 lanes)
+  int stages;              // of the ring
   int n_tiles, m_tiles;    // weight tiles, row tiles
   const float* sx;         // [rows]
   const float* sw;         // [n_out]
@@ -37,20 +39,44 @@ struct I8Args {
   int* status;
 };
 
+constexpr int kI8MaxStages = 32;
+
+// Shared memory: the barriers and the row scales, then the ring: args.stages weight slots of
+// args.box lines, 16 KB for the lanes that the last of them leaves unloaded, the rows' slots.
+// (An MMA always reads 128 lines: what it finds past a slot goes to lanes that nobody reads.)
 template <int TN>
 struct I8Config {
-  static constexpr int kABytes = kBM * kI8BK;
   static constexpr int kBBytes = TN * kI8BK;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = TN <= 32 ? 10 : (TN == 64 ? 8 : (TN == 128 ? 6 : 4));
-  static constexpr int kTmemCols = 2 * TN <= 32 ? 32 : 2 * TN;
-  static constexpr int kScaleOffset = kStages * kStageBytes;  // [4 warps][TN] row scales
-  static constexpr int kBarOffset = kScaleOffset + 4 * TN * 4;
-  static constexpr int kNumBars = 2 * kStages + 4;
-  static constexpr int kSmemBytes = kBarOffset + kNumBars * 8 + 16 + 1024;
+  static constexpr int kTmemCols = 2 * TN;
+  static constexpr int kNumBars = 2 * kI8MaxStages + 4;
+  static constexpr int kScaleOffset = kNumBars * 8 + 16;                    // [4 warps][TN] row scales
+  static constexpr int kFixedBytes = kScaleOffset + 4 * TN * 4 + 1024 + kBM * kI8BK;
+  static constexpr int kMaxBytes = 224 * 1024;
+  static constexpr int slot_bytes(int box) { return box * kI8BK + kBBytes; }
+  // as many blocks of K in flight as fit: a small tile's whole K
+  static constexpr int stages(int box, int kb) {
+    const int fit = (kMaxBytes - kFixedBytes) / slot_bytes(box);
+    const int most = fit < kI8MaxStages ? fit : kI8MaxStages;
+    return kb < 2 ? 2 : (kb < most ? kb : most);
+  }
   static_assert(TN >= 16 && TN <= 256 && (TN & (TN - 1)) == 0, "TN is a power of two in [16, 256]");
-  static_assert(kSmemBytes <= 232448, "shared memory budget");
+  static_assert(kFixedBytes + 4 * slot_bytes(kBM) <= kMaxBytes, "four stages of the largest tile fit");
 };
+
+// One lane of the (converged) warp.  Inside a branch on it the compiler knows that one thread
+// runs: the copies and MMAs there take their operands from uniform registers at once, where a
+// branch on lane == 0 costs several hundred cycles for each block of K.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(one));
+  return one != 0;
+}
 
 // D[tmem] (+)= A[smem] * B[smem]^T, signed 8-bit inputs, 32-bit integer accumulator.
 __device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -111,19 +137,17 @@ __device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float*
 }
 
 template <int TN, typename OutT>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(kI8Threads, 1)
     i8_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const I8Args args) {
   using Cfg = I8Config<TN>;
-  constexpr int S = Cfg::kStages;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = smem_u32(smem_raw);
-  const uint32_t base_addr = (raw_addr + 1023u) & ~1023u;
-  uint8_t* smem = smem_raw + (base_addr - raw_addr);
-  const uint32_t a_base = base_addr;
-  const uint32_t b_base = base_addr + S * Cfg::kABytes;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int S = args.stages;
+  const uint32_t a_bytes = (uint32_t)args.box * kI8BK;  // eight lines (1 KB) are a swizzle atom
+  const uint32_t a_base = (smem_u32(smem) + (uint32_t)(Cfg::kScaleOffset + 4 * TN * 4) + 1023u) & ~1023u;
+  const uint32_t b_base = a_base + S * a_bytes + kBM * kI8BK;
   float* scales = reinterpret_cast<float*>(smem + Cfg::kScaleOffset);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::kBarOffset);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -136,7 +160,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(full_bar(s), 1);
+      mbar_init(full_bar(s), 2);  // the weights' and the rows' producer
       mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -160,37 +184,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   const int units = args.n_tiles * args.m_tiles;  // row tiles of one weight tile next to each other
 
-  if (warp == 0) {
-    // ---------------------------------------------------------------- TMA producer
-    if (lane == 0) {
-      const uint32_t tx = (uint32_t)(args.box * kI8BK + Cfg::kBBytes);
-      // The ring's first weight tiles do not depend on the kernel that makes xq.
-      int ahead = 0;
-      if (args.early) {
-        int u = blockIdx.x, kb = 0;
-        while (ahead < S && u < units) {
-          mbar_arrive_expect_tx(full_bar(ahead), tx);
-          tma_load_2d(a_base + ahead * Cfg::kABytes, &map_w, full_bar(ahead), kb * kI8BK, u / args.m_tiles * args.box);
-          ++ahead;
-          if (++kb == args.kb) kb = 0, u += gridDim.x;
-        }
-      }
-      pdl_wait();
+  if (warp == 0 || warp == 6) {
+    // ---------------------------------------------------------------- TMA producers
+    // One warp for the weights and one for the rows: issuing a copy takes about as long as the
+    // MMAs of half a narrow tile's block.  The weights need not wait for the kernel before.
+    if (elect_one()) {
+      const bool weights = warp == 0;
+      const uint32_t bytes = weights ? a_bytes : (uint32_t)Cfg::kBBytes;
+      const uint32_t ring = weights ? a_base : b_base;
+      const CUtensorMap* map = weights ? &map_w : &map_x;
+      if (!weights || !args.early) pdl_wait();
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const int n0 = u / args.m_tiles * args.box, m0 = u % args.m_tiles * TN;
+        const int y = weights ? u / args.m_tiles * args.box : u % args.m_tiles * TN;
         for (int kb = 0; kb < args.kb; ++kb) {
-          if (issued >= ahead) {
-            if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, args.status)) {
-              ok = false;
-              break;
-            }
-            mbar_arrive_expect_tx(full_bar(stage), tx);
-            tma_load_2d(a_base + stage * Cfg::kABytes, &map_w, full_bar(stage), kb * kI8BK, n0);
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, args.status)) {
+            ok = false;
+            break;
           }
-          tma_load_2d(b_base + stage * Cfg::kBBytes, &map_x, full_bar(stage), kb * kI8BK, m0);
+          mbar_arrive_expect_tx(full_bar(stage), bytes);
+          tma_load_2d(ring + stage * bytes, map, full_bar(stage), kb * kI8BK, y);
           ++issued;
           if (++stage == S) {
             stage = 0;
@@ -199,14 +214,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       if (!ok) {
-        // Aborting: let the copies already in flight land before the CTA exits.
+        // Aborting: let the copies already in flight land before the CTA exits (their stages
+        // may lack the other producer's part: the wait is bounded).
         const int outstanding = issued < S ? issued : S;
+        const unsigned long long t0 = globaltimer_ns();
         for (int i = 0; i < outstanding; ++i) {
           if (--stage < 0) {
             stage = S - 1;
             phase ^= 1u;
           }
-          const unsigned long long t0 = globaltimer_ns();
           while (!mbar_try_wait(full_bar(stage), phase) && globaltimer_ns() - t0 < kWaitLimitNs / 20) {
           }
         }
@@ -214,7 +230,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc = make_idesc_s8_s32(kBM, TN);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
@@ -229,7 +245,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint64_t adesc = make_sw128_desc(a_base + stage * Cfg::kABytes);
+          const uint64_t adesc = make_sw128_desc(a_base + stage * a_bytes);
           const uint64_t bdesc = make_sw128_desc(b_base + stage * Cfg::kBBytes);
 #pragma unroll
           for (int k = 0; k < kI8BK / 32; ++k)  // +32 bytes per K step inside the 128-byte swizzled line
@@ -430,7 +446,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer (both CTAs)
-    if (lane == 0) {
+    if (elect_one()) {
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -480,7 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer (rank 0)
-    if (lane == 0 && leader) {
+    if (leader && elect_one()) {
       constexpr uint32_t idesc_full = make_idesc_s8_s32(2 * kBM, BN);
       const uint32_t idesc_tail = make_idesc_s8_s32(2 * kBM, BN / sched.tail_split);
       int stage = 0, acc = 0;
@@ -601,5 +617,29 @@ constexpr int kQuantThreads = 256;
 using QuantizeKernel = void (*)(const void* x, long long ld_x, int rows, int K, int8_t* q, long long ld_q, float* scale);
 // for bf16 or fp32 rows, with 16-byte loads (vec) or without
 QuantizeKernel quantize_rows_kernel_for(bool bf16, bool vec);
+
+// A few rows against all channels in one launch: each CTA quantises the rows for itself (or
+// copies quantised ones) into shared memory, then a warp takes a channel at a time with
+// dp4a (i8_kernels.cu).
+constexpr int kI8GemvThreads = 256;
+constexpr int kI8GemvCtas = 3;           // of an SM
+constexpr int kI8GemvRows = 2;           // most rows
+constexpr int kI8GemvBytes = 32768;      // most bytes of quantised rows
+enum I8Source { kI8FromInt8 = 0, kI8FromBf16 = 1, kI8FromF32 = 2 };
+struct I8GemvArgs {
+  const void* x;        // [rows, K], row stride ld_x elements
+  long long ld_x;
+  int vec;              // 16-byte loads of x
+  const float* sx;      // [rows], with int8 rows
+  const int8_t* w;
+  long long ld_w;
+  const float* sw;
+  const void* bias;
+  void* out;
+  long long ld_out;
+  int rows, K, n_out;
+};
+using I8GemvKernel = void (*)(I8GemvArgs);
+I8GemvKernel i8_gemv_kernel_for(I8Source source, bool out_bf16, int rows);
 
 }  // namespace dels

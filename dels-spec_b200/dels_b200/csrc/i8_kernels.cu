@@ -1,4 +1,5 @@
-// Rows to 8-bit integers:
+// Rows to 8-bit integers, and their product with 8-bit weights for a few rows.
+//
 //
 //   a = max_k |x[k]|,  scale = a / 127,  q[k] = rint(x[k] * (127 / a))   (half to even)
 //
@@ -32,55 +33,197 @@ __device__ __forceinline__ int to_i8(float x, float inv) {
 
 }  // namespace
 
+namespace {
+
+// 8 values of a row as int8 (what 16-byte loads give), packed.
+template <typename T>
+__device__ __forceinline__ uint2 quantize8(const T* p, float up, float inv) {
+  float v[8];
+  load8(p, v);
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    w[h] = (uint32_t)(to_i8(v[4 * h] * up, inv) & 255) | (uint32_t)(to_i8(v[4 * h + 1] * up, inv) & 255) << 8 |
+           (uint32_t)(to_i8(v[4 * h + 2] * up, inv) & 255) << 16 | (uint32_t)(to_i8(v[4 * h + 3] * up, inv) & 255) << 24;
+  return make_uint2(w[0], w[1]);
+}
+
+// One row by the whole block (kQuantThreads threads); returns its scale.  warp_top: shared,
+// a float for each warp.
+template <typename T>
+__device__ __forceinline__ float quantize_row(const T* src, int K, bool vec, int8_t* dst, float* warp_top) {
+  const int t = threadIdx.x;
+  const int whole = vec ? K / 8 * 8 : 0;
+  float top = 0.0f;
+  for (int k = t * 8; k < whole; k += kQuantThreads * 8) {
+    float v[8];
+    load8(src + k, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmax_nan(top, fabsf(v[j]));
+  }
+  for (int k = whole + t; k < K; k += kQuantThreads) top = fmax_nan(top, fabsf(to_f32(src[k])));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmax_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+  __syncthreads();  // warp_top of the row before has been read
+  if ((t & 31) == 0) warp_top[t >> 5] = top;
+  __syncthreads();
+  top = warp_top[0];
+#pragma unroll
+  for (int w = 1; w < kQuantThreads / 32; ++w) top = fmax_nan(top, warp_top[w]);
+  // 127 / top overflows for a top below 2^-121: such rows are scaled up by a power of two
+  // first, which changes no quotient
+  const float up = top < 0x1p-100f ? 0x1p100f : 1.0f;
+  const float inv = top > 0.0f && top <= 3.402823466e+38f ? __fdiv_rn(127.0f, top * up) : 0.0f;
+  for (int k = t * 8; k < whole; k += kQuantThreads * 8) *reinterpret_cast<uint2*>(dst + k) = quantize8(src + k, up, inv);
+  for (int k = whole + t; k < K; k += kQuantThreads) dst[k] = (int8_t)to_i8(to_f32(src[k]) * up, inv);
+  return __fdiv_rn(top, 127.0f);
+}
+
+}  // namespace
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const void* x, long long ld_x, int rows, int K,
                                                                       int8_t* q, long long ld_q, float* scale) {
   __shared__ float warp_top[kQuantThreads / 32];
-  const int t = threadIdx.x;
   pdl_wait();
   pdl_trigger();
   for (int row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* src = static_cast<const T*>(x) + (long long)row * ld_x;
-    int8_t* dst = q + (long long)row * ld_q;
-    const int whole = VEC ? K / 8 * 8 : 0;
-    float top = 0.0f;
-    for (int k = t * 8; k < whole; k += kQuantThreads * 8) {
-      float v[8];
-      load8(src + k, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmax_nan(top, fabsf(v[j]));
-    }
-    for (int k = whole + t; k < K; k += kQuantThreads) top = fmax_nan(top, fabsf(to_f32(src[k])));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-    __syncthreads();
-    if ((t & 31) == 0) warp_top[t >> 5] = top;
-    __syncthreads();
-    top = warp_top[0];
-#pragma unroll
-    for (int w = 1; w < kQuantThreads / 32; ++w) top = fmax_nan(top, warp_top[w]);
-    // 127 / top overflows for a top below 2^-121: such rows are scaled up by a power of two
-    // first, which changes no quotient
-    const float up = top < 0x1p-100f ? 0x1p100f : 1.0f;
-    const float inv = top > 0.0f && top <= 3.402823466e+38f ? __fdiv_rn(127.0f, top * up) : 0.0f;
-    if (t == 0) scale[row] = __fdiv_rn(top, 127.0f);
-    for (int k = t * 8; k < whole; k += kQuantThreads * 8) {
-      float v[8];
-      load8(src + k, v);
-      uint32_t w[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        w[h] = (uint32_t)(to_i8(v[4 * h] * up, inv) & 255) | (uint32_t)(to_i8(v[4 * h + 1] * up, inv) & 255) << 8 |
-               (uint32_t)(to_i8(v[4 * h + 2] * up, inv) & 255) << 16 | (uint32_t)(to_i8(v[4 * h + 3] * up, inv) & 255) << 24;
-      *reinterpret_cast<uint2*>(dst + k) = make_uint2(w[0], w[1]);
-    }
-    for (int k = whole + t; k < K; k += kQuantThreads) dst[k] = (int8_t)to_i8(to_f32(src[k]) * up, inv);
+    const float s = quantize_row(static_cast<const T*>(x) + (long long)row * ld_x, K, VEC, q + (long long)row * ld_q,
+                                 warp_top);
+    if (threadIdx.x == 0) scale[row] = s;
   }
 }
 
 QuantizeKernel quantize_rows_kernel_for(bool bf16, bool vec) {
   if (bf16) return vec ? quantize_rows_kernel<__nv_bfloat16, true> : quantize_rows_kernel<__nv_bfloat16, false>;
   return vec ? quantize_rows_kernel<float, true> : quantize_rows_kernel<float, false>;
+}
+
+// --------------------------------------------------------------------------------
+// A few rows: y[r, n] = (sum_k xq[r, k] w[n, k]) * sx[r] * sw[n] (+ bias[n]).
+// Bound by the weights' bytes.  A warp reads a channel with 16-byte loads, the next channel's
+// first ones on their way while it adds up, and multiplies by dp4a; the sum is exact.
+// --------------------------------------------------------------------------------
+namespace {
+
+__device__ __forceinline__ uint4 load_weights(const int8_t* p) {
+  uint4 w;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+               : "l"(p));
+  return w;
+}
+
+// dynamic shared memory: [ROWS][padded K] quantised rows, zero past K
+template <typename T, typename OutT, int ROWS>
+__global__ void __launch_bounds__(kI8GemvThreads, kI8GemvCtas) i8_gemv_kernel(I8GemvArgs a) {
+  constexpr int kWarps = kI8GemvThreads / 32;
+  constexpr int U = 8;  // 16-byte loads of a lane in flight
+  extern __shared__ __align__(16) int8_t rows_q[];
+  __shared__ float warp_top[kWarps], scale[ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int padded = (a.K + 15) / 16 * 16, chunks = padded / 16, whole = a.K / 16;
+  int n = blockIdx.x * kWarps + warp;
+  uint4 w[U];
+  auto fetch = [&](int channel, int c0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * 32 + lane;
+      w[u] = channel < a.n_out && c < whole ? load_weights(a.w + (long long)channel * a.ld_w + 16 * c) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  pdl_wait();  // (the kernel before this one may be the one that quantised the weights)
+  pdl_trigger();
+  fetch(n, 0);
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    int8_t* dst = rows_q + r * padded;
+    if (r >= a.rows) break;
+    if constexpr (sizeof(T) == 1) {
+      const int8_t* src = static_cast<const int8_t*>(a.x) + (long long)r * a.ld_x;
+      for (int c = threadIdx.x; c < whole; c += kI8GemvThreads)
+        reinterpret_cast<uint4*>(dst)[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+      for (int k = 16 * whole + threadIdx.x; k < a.K; k += kI8GemvThreads) dst[k] = src[k];
+      if (threadIdx.x == 0) scale[r] = a.sx[r];
+    } else {
+      const float s = quantize_row(static_cast<const T*>(a.x) + (long long)r * a.ld_x, a.K, a.vec != 0, dst, warp_top);
+      if (threadIdx.x == 0) scale[r] = s;
+    }
+    for (int k = a.K + threadIdx.x; k < padded; k += kI8GemvThreads) dst[k] = 0;
+  }
+  __syncthreads();
+  const int step = gridDim.x * kWarps;
+#pragma unroll 1
+  for (; n < a.n_out; n += step) {
+    int acc[ROWS] = {};
+    for (int c0 = 0; c0 < chunks; c0 += 32 * U) {
+      uint4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = w[u];
+      // a channel's last, partial 16 bytes come byte by byte
+      const int last = whole - c0;
+      if (whole < chunks && last >= 0 && last < 32 * U && (last & 31) == lane) {
+        const int8_t* p = a.w + (long long)n * a.ld_w + 16 * whole;
+        uint32_t b[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 15; ++j)
+          if (j < a.K - 16 * whole) b[j >> 2] |= (uint32_t)(uint8_t)p[j] << (8 * (j & 3));
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u == last >> 5) v[u] = make_uint4(b[0], b[1], b[2], b[3]);
+      }
+      const bool more = c0 + 32 * U < chunks;
+      fetch(more ? n : n + step, more ? c0 + 32 * U : 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + u * 32 + lane;
+        if (c < chunks) {
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) {
+            if (r >= a.rows) break;
+            const uint4 x = reinterpret_cast<const uint4*>(rows_q + r * padded)[c];
+            acc[r] = __dp4a((int)v[u].x, (int)x.x, acc[r]);
+            acc[r] = __dp4a((int)v[u].y, (int)x.y, acc[r]);
+            acc[r] = __dp4a((int)v[u].z, (int)x.z, acc[r]);
+            acc[r] = __dp4a((int)v[u].w, (int)x.w, acc[r]);
+          }
+        }
+      }
+    }
+    int mine = 0;  // lane r: the sum of row r
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int total = __reduce_add_sync(0xffffffffu, acc[r]);
+      mine = lane == r ? total : mine;
+    }
+    if (lane < a.rows) {
+      float y = __int2float_rn(mine) * scale[lane] * __ldg(a.sw + n);
+      if (a.bias != nullptr) y += to_f32(static_cast<const OutT*>(a.bias)[n]);
+      OutT* out = static_cast<OutT*>(a.out) + (long long)lane * a.ld_out + n;
+      if constexpr (sizeof(OutT) == 2)
+        *out = __float2bfloat16_rn(y);
+      else
+        *out = y;
+    }
+  }
+}
+
+template <typename T, typename OutT>
+I8GemvKernel i8_gemv_rows(int rows) {
+  return rows <= 1 ? i8_gemv_kernel<T, OutT, 1> : i8_gemv_kernel<T, OutT, 2>;
+}
+
+}  // namespace
+
+I8GemvKernel i8_gemv_kernel_for(I8Source source, bool out_bf16, int rows) {
+  switch (source) {
+    case kI8FromInt8:
+      return out_bf16 ? i8_gemv_rows<int8_t, __nv_bfloat16>(rows) : i8_gemv_rows<int8_t, float>(rows);
+    case kI8FromBf16:
+      return out_bf16 ? i8_gemv_rows<__nv_bfloat16, __nv_bfloat16>(rows) : i8_gemv_rows<__nv_bfloat16, float>(rows);
+    default:
+      return out_bf16 ? i8_gemv_rows<float, __nv_bfloat16>(rows) : i8_gemv_rows<float, float>(rows);
+  }
 }
 
 }  // namespace dels
