@@ -890,13 +890,14 @@ int launch_i8_pair(const void* xq, long long ld_x, const void* wq, long long ld_
   a.m_tiles = cdiv(a.rows, Cfg::BN);
   a.n_tiles = cdiv(a.n_out, 2 * kBM);
   a.kb = cdiv(K, kI8BK);
-  a.tail = kScorerTailSplit;
+  a.bn = cdiv(cdiv(a.rows, a.m_tiles), 32) * 32;
+  a.tail = a.bn % 128 == 0 ? 4 : (a.bn % 64 == 0 ? 2 : 1);  // split tiles are multiples of 32, too
   const long long tiles = (long long)a.m_tiles * a.n_tiles;
   const long long want = tiles < max_pairs ? tiles * a.tail : tiles;
   CUtensorMap mw, mx, mxt;
   if ((rc = make_map_i8(&mw, wq, K, a.n_out, ld_w, kBM)) != DELS_OK) return rc;
-  if ((rc = make_map_i8(&mx, xq, K, a.rows, ld_x, Cfg::BN / 2)) != DELS_OK) return rc;
-  if ((rc = make_map_i8(&mxt, xq, K, a.rows, ld_x, Cfg::BN / 2 / a.tail)) != DELS_OK) return rc;
+  if ((rc = make_map_i8(&mx, xq, K, a.rows, ld_x, a.bn / 2)) != DELS_OK) return rc;
+  if ((rc = make_map_i8(&mxt, xq, K, a.rows, ld_x, a.bn / 2 / a.tail)) != DELS_OK) return rc;
   DELS_CHECK_PDL("i8_pair_kernel launch",
                  launch_pdl(i8_pair_kernel<OutT>, dim3((unsigned)(2 * (want < max_pairs ? want : max_pairs))),
                             dim3(kTcThreads), Cfg::kSmemBytes, st, mw, mx, mxt, a));
@@ -908,10 +909,11 @@ int launch_i8_out(const void* xq, long long ld_x, const void* wq, long long ld_w
                   int max_pairs, cudaStream_t st) {
   const I8Shape shape = plan_i8(a.rows, a.n_out, sm_count);
   if (a.rows > kBM && max_pairs > 0 && g_use_pairs) {
-    // Pairs where their large tiles fill the device: a pair's block of K costs what a 256-row
+    // Pairs where their large tiles fill the device: a pair's block of K costs what a bn-row
     // tile's does.
-    const long long tiles = (long long)cdiv(a.rows, I8PairConfig::BN) * cdiv(a.n_out, 2 * kBM);
-    if (cdiv(tiles, max_pairs) * (32ll + 256) <= shape.cost + shape.cost / 8)
+    const int m_tiles = cdiv(a.rows, I8PairConfig::BN), bn = cdiv(cdiv(a.rows, m_tiles), 32) * 32;
+    const long long tiles = (long long)m_tiles * cdiv(a.n_out, 2 * kBM);
+    if (cdiv(tiles, max_pairs) * (32ll + 128 + bn / 2) <= shape.cost + shape.cost / 8)
       return launch_i8_pair<OutT>(xq, ld_x, wq, ld_w, K, a, max_pairs, st);
   }
   switch (shape.tn) {

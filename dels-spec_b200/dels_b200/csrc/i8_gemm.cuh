@@ -34,7 +34,7 @@ struct I8Args {
   void* out;               // [rows, n_out] bf16 or fp32
   long long ld_out;
   int store2;              // bf16: two channels per store (even ld_out, 4-byte aligned out)
-  int tail;                // i8_pair_kernel: ways a tile of the last wave is split along the rows
+  int bn, tail;            // i8_pair_kernel: rows of a tile, ways one of the last wave is split along them
   int early;               // the weights are not written by the previous kernel: load them before waiting for it
   int* status;
 };
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 
 // --------------------------------------------------------------------------------
 // The same product on CTA pairs (tcgen05.mma.cta_group::2), for more than 128 rows: a tile is
-// 256 channels x 256 rows, each CTA stages its 128 channels and half of the rows' tile, so a
+// 256 channels x up to 256 rows (a multiple of 32 that the rows fill well), each CTA stages its 128 channels and half of the rows' tile, so a
 // block of K moves 32 KB through each SM's shared memory for the work that takes 48 KB in
 // i8_gemm_kernel.  The barriers are those of tc_scorer_pair_kernel: rank 0 issues the MMAs of
 // both CTAs, whose copies complete on rank 0's full barriers.  Two blocks of K form a stage
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 // rows (make_schedule's tail).
 // --------------------------------------------------------------------------------
 struct I8PairConfig {
-  static constexpr int BN = 256;                 // rows of a tile
+  static constexpr int BN = 256;                 // most rows of a tile
   static constexpr int kGroup = 2;               // blocks of K in a stage
   static constexpr int kABytes = kBM * kI8BK;
   static constexpr int kBBytes = BN / 2 * kI8BK;
@@ -383,7 +383,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     i8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const __grid_constant__ CUtensorMap map_xt, const I8Args args) {
   using Cfg = I8PairConfig;
-  constexpr int S = Cfg::kStages, KG = Cfg::kGroup, BN = Cfg::BN;
+  constexpr int S = Cfg::kStages, KG = Cfg::kGroup;
+  const int BN = args.bn;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base_addr = (raw_addr + 1023u) & ~1023u;
@@ -497,7 +498,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer (rank 0)
     if (leader && elect_one()) {
-      constexpr uint32_t idesc_full = make_idesc_s8_s32(2 * kBM, BN);
+      const uint32_t idesc_full = make_idesc_s8_s32(2 * kBM, BN);
       const uint32_t idesc_tail = make_idesc_s8_s32(2 * kBM, BN / sched.tail_split);
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
@@ -506,7 +507,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         const uint32_t idesc = u >= sched.main_units ? idesc_tail : idesc_full;
         if (!mbar_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, args.status)) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN);
+        const uint32_t d_tmem = tmem_base + (uint32_t)(acc * Cfg::BN);
         for (int kb = 0; kb < args.kb; kb += KG) {
           if (!mbar_wait(full_bar(stage), phase, abort_flag, args.status)) {
             ok = false;
@@ -546,7 +547,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
   } else {
     // ---------------------------------------------------------------- epilogue (both CTAs)
     const int quad = warp & 3;
-    float* scale = scales + quad * BN;
+    float* scale = scales + quad * Cfg::BN;
     const uint32_t tempty_leader0 = mapa_shared(tempty_bar(0), 0);
     const uint32_t tempty_leader1 = mapa_shared(tempty_bar(1), 0);
     OutT* out = static_cast<OutT*>(args.out);
@@ -576,7 +577,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       }
       if (!mbar_wait(tfull_bar(acc), acc_phase, abort_flag, args.status)) break;
       tc_fence_after();
-      const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * BN);
+      const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(acc * Cfg::BN);
       OutT* dst = out + (long long)m0 * args.ld_out + n;
 #pragma unroll 1
       for (int c = 0; c < (warp_ok ? valid : 0); c += 32) {

@@ -101,6 +101,8 @@ def check_product(got, xq, wq, sx, sw, bias):
     (1, 1, 1), (1, 16, 8), (2, 127, 7), (5, 128, 129), (16, 129, 64), (17, 100, 1003), (32, 512, 2000), (33, 2561, 77),
     (64, 256, 5001), (65, 4096, 256), (128, 384, 640), (129, 1000, 333), (256, 130, 1300), (513, 640, 1026),
     (1, 4096, 20011), (300, 3000, 2),
+    # enough tiles for CTA pairs: tiles of 160, 192 and 256 rows, a last wave split along the rows
+    (129, 200, 38001), (300, 256, 30000), (513, 130, 19001), (512, 384, 20480),
 ])
 def test_product_is_exact(cuda_device, out_dtype, rows, K, N):
     from dels_b200 import ops
