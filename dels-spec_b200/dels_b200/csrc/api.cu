@@ -289,10 +289,10 @@ int init_device(int dev) {
     SET(gru_finalize_kernel, 0);
     SET(wait_selftest_kernel, 0);
     SET_SHARED(beam_reorder_kernel, 0);
-    for (int i = 0; i < 8; ++i) {
-      const bool bf16 = (i & 4) != 0, mix = (i & 2) != 0, vec = (i & 1) != 0;
-      SET_SHARED(beam_scan_kernel_for(bf16, mix, vec), vec ? kBeamScanSmemMax : 0);
-      SET_SHARED(beam_finish_kernel_for(bf16, mix, vec), kBeamFinishSmemMax);
+    for (int i = 0; i < 4; ++i) {
+      const bool bf16 = (i & 2) != 0, vec = (i & 1) != 0;
+      SET_SHARED(beam_scan_kernel_for(bf16, vec), vec ? kBeamScanSmemMax : 0);
+      SET_SHARED(beam_finish_kernel_for(bf16, vec), kBeamFinishSmemMax);
       SET(quantize_rows_kernel_for(bf16, vec), 0);
     }
     for (int i = 0; i < 12; ++i)
@@ -725,15 +725,16 @@ int fused_argmax_common(const void* h, long long ld_h, const void* W, long long 
 
 // Plans a selection's scan and lays out its scratch over `base` (counted only when `a` is
 // null); returns the scratch's bytes.
-size_t beam_plan(int n_seq, int beams, int V, int elem, bool mix, int sm_count, char* base, BeamSelectArgs* a) {
+size_t beam_plan(int n_seq, int beams, int V, int elem, bool shared, int sm_count, char* base, BeamSelectArgs* a) {
   const size_t rows = (size_t)n_seq * beams;
   const int groups = cdiv(V, kBeamGroup);
-  const int scan_rows = mix ? (beams < kBeamScanRows ? beams : kBeamScanRows) : 1;
-  const int blocks = n_seq * cdiv(beams, scan_rows);
+  const int run_rows = shared ? beams : (int)rows;
+  const int scan_rows = run_rows < kBeamScanRows ? run_rows : kBeamScanRows;
+  const int blocks = (int)(rows / run_rows) * cdiv(run_rows, scan_rows);
   // As many CTAs as the device holds at once, by the shared memory of an SM and the kernel's
   // registers, with a group for each of their teams at least.
-  const int smem = beam_scan_smem(scan_rows, elem, mix) + 2048;
-  const int fit = (220 << 10) / smem, most = mix ? 5 : 8;
+  const int smem = beam_scan_smem(scan_rows, elem, shared) + 2048;
+  const int fit = (220 << 10) / smem, most = kBeamScanCtas;
   const long long units = (long long)blocks * groups;
   const long long teams = scan_teams(scan_rows);
   long long ctas = (long long)(fit < most ? fit : most) * sm_count;
@@ -745,6 +746,7 @@ size_t beam_plan(int n_seq, int beams, int V, int elem, bool mix, int sm_count, 
   if (a != nullptr) {
     a->groups = groups;
     a->parts = parts;
+    a->run_rows = run_rows;
     a->scan_rows = scan_rows;
     a->scan_ctas = (int)ctas;
     a->share.per = (int)(units / ctas);
@@ -755,13 +757,13 @@ size_t beam_plan(int n_seq, int beams, int V, int elem, bool mix, int sm_count, 
   return part0 + align256(rows * parts * sizeof(float2));
 }
 
-int launch_beam_select(BeamSelectArgs a, bool bf16, bool mix, bool vec, cudaStream_t st) {
+int launch_beam_select(BeamSelectArgs a, bool bf16, bool shared, bool vec, cudaStream_t st) {
   const int elem = bf16 ? 2 : 4;
-  a.slot_bytes = beam_slot_bytes(a.scan_rows, elem, mix);
+  a.slot_bytes = beam_slot_bytes(a.scan_rows, elem, shared);
   DELS_CHECK_PDL("beam_scan_kernel launch",
-                 launch_pdl(beam_scan_kernel_for(bf16, mix, vec), dim3((unsigned)a.scan_ctas),
+                 launch_pdl(beam_scan_kernel_for(bf16, vec), dim3((unsigned)a.scan_ctas),
                             dim3(32 * scan_pairs(a.scan_rows) * scan_teams(a.scan_rows)),
-                            vec ? beam_scan_smem(a.scan_rows, elem, mix) : 0, st, a));
+                            vec ? beam_scan_smem(a.scan_rows, elem, shared) : 0, st, a));
   // Sixteen warps or nearly: several share a beam's groups where there are few beams.  The bound
   // needs some more maxima than candidates: a lane offers its four quarters' where its
   // largest alone would be too few.
@@ -771,7 +773,7 @@ int launch_beam_select(BeamSelectArgs a, bool bf16, bool mix, bool vec, cudaStre
   a.finish_values = a.beams * lanes < 4 * a.select ? 4 : 1;
   const int warps = split * (a.beams < kBeamFinishWarps ? a.beams : kBeamFinishWarps);
   DELS_CHECK_PDL("beam_finish_kernel launch",
-                 launch_pdl(beam_finish_kernel_for(bf16, mix, vec), dim3((unsigned)a.n_seq), dim3(32 * warps),
+                 launch_pdl(beam_finish_kernel_for(bf16, vec), dim3((unsigned)a.n_seq), dim3(32 * warps),
                             beam_finish_smem(a.beams, a.select, warps, a.beams * split * 32 * a.finish_values), st, a));
   return DELS_OK;
 }
@@ -1699,10 +1701,10 @@ int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const voi
   // with a whole load
   const bool vec = V % 8 == 0 && aligned16(logits) && (ld_logits * elem) % 16 == 0 &&
                    (base == nullptr || (aligned16(base) && (ld_base * elem) % 16 == 0)) && aligned16(prior);
-  const bool mix = base != nullptr || prior != nullptr;
-  beam_plan(n_seq, beams, V, (int)elem, mix, ds->sm_count < kMaxSmCount ? ds->sm_count : kMaxSmCount,
+  const bool shared = base != nullptr || prior != nullptr;
+  beam_plan(n_seq, beams, V, (int)elem, shared, ds->sm_count < kMaxSmCount ? ds->sm_count : kMaxSmCount,
             static_cast<char*>(ws) + DELS_WS_HEADER_BYTES, &a);
-  return launch_beam_select(a, dtype == DELS_DTYPE_BF16, mix, vec, reinterpret_cast<cudaStream_t>(stream));
+  return launch_beam_select(a, dtype == DELS_DTYPE_BF16, shared, vec, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t* parents, int n_seq, int beams,

@@ -144,26 +144,63 @@ struct Shared {
   float nbeta;  // -beta
 };
 
+template <typename T>
+__device__ __forceinline__ Shared<T> shared_terms(const BeamSelectArgs& a, int seq) {
+  Shared<T> sh{nullptr, nullptr, 0.0f};
+  if (a.base != nullptr) sh.base = static_cast<const T*>(a.base) + (long long)seq * a.ld_base;
+  if (a.prior != nullptr) sh.prior = a.prior, sh.nbeta = -__ldg(a.beta);
+  return sh;
+}
+
 // x = (base + logit) - beta prior, every operation rounded by itself.
-template <typename T, bool MIX>
+template <typename T>
 __device__ __forceinline__ float mixed_logit(const T* row, const Shared<T>& sh, int v) {
   float x = to_f32(row[v]);
-  if constexpr (MIX) {
-    if (sh.base != nullptr) x = __fadd_rn(to_f32(sh.base[v]), x);
-    if (sh.prior != nullptr) x = __fadd_rn(x, __fmul_rn(sh.nbeta, __ldg(sh.prior + v)));
-  }
+  if (sh.base != nullptr) x = __fadd_rn(to_f32(sh.base[v]), x);
+  if (sh.prior != nullptr) x = __fadd_rn(x, __fmul_rn(sh.nbeta, __ldg(sh.prior + v)));
   return x;
 }
 
-// A lane's logits of the group at v0 without 16-byte loads; -inf past V.
-template <typename T, bool MIX>
-__device__ __forceinline__ void load_single(const T* row, const Shared<T>& sh, int v0, int V, int lane,
-                                            float2 (&x)[kPer / 2]) {
+// A lane's logits of the group at v0 of two rows without 16-byte loads; -inf past V.  In a
+// whole group all loads leave before the first of them is used.
+template <typename T>
+__device__ __forceinline__ void load_single(const T* const (&row)[2], const Shared<T>& sh, int v0, int V, int lane,
+                                            float2 (&x)[2][kPer / 2]) {
+  if (v0 + kBeamGroup <= V) {
+    T w[2][kPer], b[kPer];
+    float p[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int v = v0 + 32 * j + lane;
+      w[0][j] = row[0][v], w[1][j] = row[1][v];
+    }
+    if (sh.base != nullptr) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) b[j] = sh.base[v0 + 32 * j + lane];
+    }
+    if (sh.prior != nullptr) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) p[j] = __ldg(sh.prior + v0 + 32 * j + lane);
+    }
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        x[r][i] = make_float2(to_f32(w[r][2 * i]), to_f32(w[r][2 * i + 1]));
+        if (sh.base != nullptr) x[r][i] = add2(make_float2(to_f32(b[2 * i]), to_f32(b[2 * i + 1])), x[r][i]);
+        if (sh.prior != nullptr)
+          x[r][i] = add2(x[r][i], mul2(make_float2(sh.nbeta, sh.nbeta), make_float2(p[2 * i], p[2 * i + 1])));
+      }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < kPer / 2; ++i) {
     const int u = v0 + 64 * i + lane, v = u + 32;
-    x[i].x = u < V ? mixed_logit<T, MIX>(row, sh, u) : neg_inf();
-    x[i].y = v < V ? mixed_logit<T, MIX>(row, sh, v) : neg_inf();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      x[r][i].x = u < V ? mixed_logit<T>(row[r], sh, u) : neg_inf();
+      x[r][i].y = v < V ? mixed_logit<T>(row[r], sh, v) : neg_inf();
+    }
   }
 }
 
@@ -207,17 +244,16 @@ __device__ __forceinline__ void fold_group(const float2 (&x)[N][kPer / 2], float
 }  // namespace
 
 // ------------------------------------------------------------------ the scan
-// A block of rows is one row, or (MIX) up to kBeamScanRows beams of a sequence, which meet
-// the draft logits and prior they share in one CTA.  A team of warps scans a group, two rows
-// a warp; the teams of a CTA take turns at the groups of its run: of one block, or of the end
+// A block is up to kBeamScanRows rows, of one sequence where its beams share draft logits or a
+// prior, which they then meet in one CTA.  A team of warps scans a group, two rows a warp; the teams of a CTA take turns at the groups of its run: of one block, or of the end
 // of one and the start of the next.  Each row's (m, S) of a CTA's share goes to part[row][CTA
 // - first CTA of the block].  With VEC a team has the next groups copied into its ring in
 // shared memory ahead of its arithmetic (bulk copies: no registers held, a handful of
 // instructions a group).
-template <typename T, bool MIX, bool VEC>
-__global__ void __launch_bounds__(32 * kBeamScanWarps, MIX ? 5 : 8) beam_scan_kernel(BeamSelectArgs a) {
-  constexpr int D = beam_scan_depth(sizeof(T), MIX);
-  constexpr int N = MIX ? 2 : 1;  // rows of a warp
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(32 * kBeamScanWarps, kBeamScanCtas) beam_scan_kernel(BeamSelectArgs a) {
+  constexpr int D = beam_scan_depth(sizeof(T));
+  constexpr int N = 2;  // rows of a warp
   extern __shared__ __align__(16) char smem[];
   __shared__ float2 team_part[kBeamScanWarps][kBeamScanRows];
   __shared__ uint64_t full[kBeamScanWarps][D], empty[kBeamScanWarps][D];  // [team][slot]
@@ -225,18 +261,16 @@ __global__ void __launch_bounds__(32 * kBeamScanWarps, MIX ? 5 : 8) beam_scan_ke
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pairs = scan_pairs(a.scan_rows), teams = (blockDim.x >> 5) / pairs;
   const int team = warp / pairs, pair = warp % pairs;
-  const int blocks_per_seq = (a.beams + a.scan_rows - 1) / a.scan_rows;
+  const int run_blocks = (a.run_rows + a.scan_rows - 1) / a.scan_rows;
   int unit = a.share.first(blockIdx.x);
   const int unit_end = a.share.first(blockIdx.x + 1);
   char* ring = smem + team * D * a.slot_bytes;
-  if (threadIdx.x == 0) {
-    aborted = 0;
-    for (int i = 0; i < kBeamScanWarps * D; ++i) {
-      mbar_init(smem_u32(&full[0][0] + i), 1);
-      mbar_init(smem_u32(&empty[0][0] + i), pairs);
-    }
+  if (VEC && threadIdx.x < kBeamScanWarps * D) {
+    mbar_init(smem_u32(&full[0][0] + threadIdx.x), 1);
+    mbar_init(smem_u32(&empty[0][0] + threadIdx.x), pairs);
     mbar_fence_init();
   }
+  if (threadIdx.x == 0) aborted = 0;
   __syncthreads();
   pdl_wait();
   int slot = 0, fill_slot = 0;
@@ -246,25 +280,23 @@ __global__ void __launch_bounds__(32 * kBeamScanWarps, MIX ? 5 : 8) beam_scan_ke
     const int block = unit / a.groups, g_begin = unit - block * a.groups;
     const int g_end = min(a.groups, g_begin + (unit_end - unit));
     unit += g_end - g_begin;
-    const int seq = block / blocks_per_seq;
-    const int row0 = seq * a.beams + block % blocks_per_seq * a.scan_rows;
-    const int n_rows = min(a.scan_rows, (seq + 1) * a.beams - row0);
+    const int run = block / run_blocks;
+    const int row0 = run * a.run_rows + block % run_blocks * a.scan_rows;
+    const int n_rows = min(a.scan_rows, (run + 1) * a.run_rows - row0);
     const T* logits = static_cast<const T*>(a.logits) + (long long)row0 * a.ld;
     // the rows to scan: lane i < n_live holds the i-th one
     const bool mine = lane < n_rows && (a.finished == nullptr || a.finished[row0 + lane] == 0);
     const uint32_t live = __ballot_sync(kAllLanes, mine);
     const int n_live = __popc(live);
     if (n_live == 0) continue;
-    int my_row = 0;
-#pragma unroll
-    for (int r = 0; r < kBeamScanRows; ++r)
-      if (((live >> r) & 1u) && __popc(live & ((1u << r) - 1u)) == lane) my_row = r;
-    const int n_mine = min(N, n_live - N * pair);  // rows of this warp, from the N pair-th on
-    Shared<T> sh{nullptr, nullptr, 0.0f};
-    if constexpr (MIX) {
-      if (a.base != nullptr) sh.base = static_cast<const T*>(a.base) + (long long)seq * a.ld_base;
-      if (a.prior != nullptr) sh.prior = a.prior, sh.nbeta = -__ldg(a.beta);
+    int my_row = lane;
+    if (n_live < n_rows) {
+#pragma unroll 1
+      for (int r = 0; r < n_rows; ++r)
+        if (((live >> r) & 1u) && __popc(live & ((1u << r) - 1u)) == lane) my_row = r;
     }
+    const int n_mine = min(N, n_live - N * pair);  // rows of this warp, from the N pair-th on
+    const Shared<T> sh = shared_terms<T>(a, run);  // (without shared terms there is one run)
     float m[N];
     float2 s[N];
     float4* tops[N];
@@ -282,10 +314,8 @@ __global__ void __launch_bounds__(32 * kBeamScanWarps, MIX ? 5 : 8) beam_scan_ke
     const char* src = nullptr;
     uint32_t src_elem = sizeof(T);
     if (lane < n_live) src = reinterpret_cast<const char*>(logits + my_row * a.ld);
-    if constexpr (MIX) {
-      if (lane == n_live && sh.base != nullptr) src = reinterpret_cast<const char*>(sh.base);
-      if (lane == n_live + 1 && sh.prior != nullptr) src = reinterpret_cast<const char*>(sh.prior), src_elem = 4;
-    }
+    if (lane == n_live && sh.base != nullptr) src = reinterpret_cast<const char*>(sh.base);
+    if (lane == n_live + 1 && sh.prior != nullptr) src = reinterpret_cast<const char*>(sh.prior), src_elem = 4;
     const uint32_t token_bytes = __reduce_add_sync(kAllLanes, src != nullptr ? src_elem : 0u);
     const uint32_t dst = smem_u32(ring) + lane * kBeamGroup * sizeof(T);
     auto copy = [&](int k) {
@@ -323,23 +353,21 @@ __global__ void __launch_bounds__(32 * kBeamScanWarps, MIX ? 5 : 8) beam_scan_ke
       if constexpr (VEC) {
 #pragma unroll
         for (int r = 0; r < N; ++r) staged(p + (N * pair + (r < n_mine ? r : 0)) * kBeamGroup, lane, x[r]);
-        if constexpr (MIX) {
-          float2 y[kPer / 2];
-          if (sh.base != nullptr) {
-            staged(p + n_live * kBeamGroup, lane, y);
+        float2 y[kPer / 2];
+        if (sh.base != nullptr) {
+          staged(p + n_live * kBeamGroup, lane, y);
 #pragma unroll
-            for (int i = 0; i < kPer / 2; ++i)
+          for (int i = 0; i < kPer / 2; ++i)
 #pragma unroll
-              for (int r = 0; r < N; ++r) x[r][i] = add2(y[i], x[r][i]);
-          }
-          if (sh.prior != nullptr) {
-            staged(reinterpret_cast<const float*>(p + (n_live + 1) * kBeamGroup), lane, y);
+            for (int r = 0; r < N; ++r) x[r][i] = add2(y[i], x[r][i]);
+        }
+        if (sh.prior != nullptr) {
+          staged(reinterpret_cast<const float*>(p + (n_live + 1) * kBeamGroup), lane, y);
 #pragma unroll
-            for (int i = 0; i < kPer / 2; ++i) {
-              y[i] = mul2(make_float2(sh.nbeta, sh.nbeta), y[i]);
+          for (int i = 0; i < kPer / 2; ++i) {
+            y[i] = mul2(make_float2(sh.nbeta, sh.nbeta), y[i]);
 #pragma unroll
-              for (int r = 0; r < N; ++r) x[r][i] = add2(x[r][i], y[i]);
-            }
+            for (int r = 0; r < N; ++r) x[r][i] = add2(x[r][i], y[i]);
           }
         }
         __syncwarp();
@@ -353,8 +381,7 @@ __global__ void __launch_bounds__(32 * kBeamScanWarps, MIX ? 5 : 8) beam_scan_ke
             }
         }
       } else {
-#pragma unroll
-        for (int r = 0; r < N; ++r) load_single<T, MIX>(row[r], sh, g * kBeamGroup, a.V, lane, x[r]);
+        load_single<T>(row, sh, g * kBeamGroup, a.V, lane, x);
       }
       float4 t[N];
       fold_group<N>(x, m, s, t);
@@ -456,7 +483,7 @@ struct RowScratch {
 // The row's `select` best logits by exact counting, however many are equal or crowd together
 // in a few groups, into w.list.  The `select` best groups by (maximum, lowest group) hold
 // them: a logit outside is beaten by one in each of those.
-template <typename T, bool MIX>
+template <typename T>
 __device__ __noinline__ void row_best_exact(const BeamSelectArgs& a, const T* logits, const Shared<T>& sh,
                                             const float4* tops, const RowScratch& w) {
   const int n_groups = min(a.select, a.groups);
@@ -470,7 +497,7 @@ __device__ __noinline__ void row_best_exact(const BeamSelectArgs& a, const T* lo
   const int last = a.V - w.quarters[n_groups - 1] * kBeamGroup;
   const int total = (n_groups - 1) * kBeamGroup + min(kBeamGroup, last);
   auto token = [&](int p) { return w.quarters[p / kBeamGroup] * kBeamGroup + p % kBeamGroup; };
-  warp_top(total, a.select, [&](int p) { return ordered_u32(mixed_logit<T, MIX>(logits, sh, token(p))); },
+  warp_top(total, a.select, [&](int p) { return ordered_u32(mixed_logit<T>(logits, sh, token(p))); },
            [&](int slot, int p, uint32_t k) { w.list[slot] = entry_key(k, token(p)); });
 }
 
@@ -495,7 +522,7 @@ __device__ __forceinline__ uint32_t warp_bound(const uint32_t (&top)[4], int n) 
 // Four logits of a lane from a quarter; -inf past V.  The loads of the logits and of what they
 // share leave together, before the first of them is used (volatile: in the order written), since
 // each may take a microsecond to come.
-template <typename T, bool MIX, bool VEC>
+template <typename T, bool VEC>
 __device__ __forceinline__ void load_quarter(const BeamSelectArgs& a, const T* logits, const Shared<T>& sh, int quarter,
                                              int lane, float2 (&x)[2]) {
   const int v = (quarter >> 2) * kBeamGroup + quarter_offset<VEC>(quarter & 3, lane, 0);
@@ -504,34 +531,30 @@ __device__ __forceinline__ void load_quarter(const BeamSelectArgs& a, const T* l
     Raw4<T> p, b;
     Raw4<float> pr;
     p.load(logits + u);
-    if constexpr (MIX) {
-      b.load((sh.base != nullptr ? sh.base : logits) + u);
-      if (sh.prior != nullptr) pr.load(sh.prior + u);
-    }
+    if (sh.base != nullptr) b.load(sh.base + u);
+    if (sh.prior != nullptr) pr.load(sh.prior + u);
     p.unpack(x);
-    if constexpr (MIX) {
-      float2 y[2];
-      if (sh.base != nullptr) {
-        b.unpack(y);
-        x[0] = add2(y[0], x[0]), x[1] = add2(y[1], x[1]);
-      }
-      if (sh.prior != nullptr) {
-        const float2 nb = make_float2(sh.nbeta, sh.nbeta);
-        pr.unpack(y);
-        x[0] = add2(x[0], mul2(nb, y[0])), x[1] = add2(x[1], mul2(nb, y[1]));
-      }
+    float2 y[2];
+    if (sh.base != nullptr) {
+      b.unpack(y);
+      x[0] = add2(y[0], x[0]), x[1] = add2(y[1], x[1]);
+    }
+    if (sh.prior != nullptr) {
+      const float2 nb = make_float2(sh.nbeta, sh.nbeta);
+      pr.unpack(y);
+      x[0] = add2(x[0], mul2(nb, y[0])), x[1] = add2(x[1], mul2(nb, y[1]));
     }
     if (v >= a.V) x[0] = x[1] = make_float2(neg_inf(), neg_inf());
   } else {
-    x[0].x = v < a.V ? mixed_logit<T, MIX>(logits, sh, v) : neg_inf();
-    x[0].y = v + 32 < a.V ? mixed_logit<T, MIX>(logits, sh, v + 32) : neg_inf();
-    x[1].x = v + 64 < a.V ? mixed_logit<T, MIX>(logits, sh, v + 64) : neg_inf();
-    x[1].y = v + 96 < a.V ? mixed_logit<T, MIX>(logits, sh, v + 96) : neg_inf();
+    x[0].x = v < a.V ? mixed_logit<T>(logits, sh, v) : neg_inf();
+    x[0].y = v + 32 < a.V ? mixed_logit<T>(logits, sh, v + 32) : neg_inf();
+    x[1].x = v + 64 < a.V ? mixed_logit<T>(logits, sh, v + 64) : neg_inf();
+    x[1].y = v + 96 < a.V ? mixed_logit<T>(logits, sh, v + 96) : neg_inf();
   }
 }
 
 // take(x, quarter) for each listed quarter.
-template <typename T, bool MIX, bool VEC, typename Take>
+template <typename T, bool VEC, typename Take>
 __device__ __forceinline__ void each_quarter(const BeamSelectArgs& a, const T* logits, const Shared<T>& sh,
                                              const int* quarters, int n_list, Take take) {
   const int lane = threadIdx.x & 31;
@@ -539,8 +562,8 @@ __device__ __forceinline__ void each_quarter(const BeamSelectArgs& a, const T* l
   for (int i = 0; i < n_list; i += 2) {  // two in flight
     float2 x[2], y[2];
     const int p = quarters[i], q = quarters[min(i + 1, n_list - 1)];
-    load_quarter<T, MIX, VEC>(a, logits, sh, p, lane, x);
-    load_quarter<T, MIX, VEC>(a, logits, sh, q, lane, y);
+    load_quarter<T, VEC>(a, logits, sh, p, lane, x);
+    load_quarter<T, VEC>(a, logits, sh, q, lane, y);
     take(x, p);
     if (i + 1 < n_list) take(y, q);
   }
@@ -548,7 +571,7 @@ __device__ __forceinline__ void each_quarter(const BeamSelectArgs& a, const T* l
 
 // The row's `select` best logits or a few more, in any order, into w.list; returns their
 // number.
-template <typename T, bool MIX, bool VEC>
+template <typename T, bool VEC>
 __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits, const Shared<T>& sh,
                                         const float4* tops, const RowScratch& w) {
   const int lane = threadIdx.x & 31;
@@ -568,7 +591,7 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
   } else {
     for (int i = lane; i < 4 * a.groups; i += 32) w.quarters[i] = i;  // at most 2 select of them
     __syncwarp();
-    each_quarter<T, MIX, VEC>(a, logits, sh, w.quarters, 4 * a.groups, [&](const float2(&x)[2], int) {
+    each_quarter<T, VEC>(a, logits, sh, w.quarters, 4 * a.groups, [&](const float2(&x)[2], int) {
       top[0] = max(top[0], ordered_u32(x[0].x)), top[1] = max(top[1], ordered_u32(x[0].y));
       top[2] = max(top[2], ordered_u32(x[1].x)), top[3] = max(top[3], ordered_u32(x[1].y));
     });
@@ -600,7 +623,7 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
   if (lane == 0) *w.count = 0;
   __syncwarp();
   if (n_list <= kBeamListCap) {
-    each_quarter<T, MIX, VEC>(a, logits, sh, w.quarters, n_list, [&](const float2(&x)[2], int q) {
+    each_quarter<T, VEC>(a, logits, sh, w.quarters, n_list, [&](const float2(&x)[2], int q) {
       uint32_t reach = (x[0].x < floor ? 0u : 1u) | (x[0].y < floor ? 0u : 2u) | (x[1].x < floor ? 0u : 4u) |
                        (x[1].y < floor ? 0u : 8u);
 #pragma unroll 1
@@ -619,7 +642,7 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
 #pragma unroll 1
       for (int v0 = 0; v0 < a.V && c < a.select; v0 += 32) {
         const int v = v0 + lane;
-        const bool masked = v < a.V && mixed_logit<T, MIX>(logits, sh, v) == neg_inf();
+        const bool masked = v < a.V && mixed_logit<T>(logits, sh, v) == neg_inf();
         const uint32_t take = __ballot_sync(kAllLanes, masked);
         const int slot = c + __popc(take & ((1u << lane) - 1u));
         if (masked) w.list[slot] = entry_key(none, v);  // slot < select + 32 <= kBeamListCap
@@ -629,7 +652,7 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
     }
     if (c >= a.select && c <= kBeamListCap) return c;
   }
-  row_best_exact<T, MIX>(a, logits, sh, tops, w);
+  row_best_exact<T>(a, logits, sh, tops, w);
   return a.select;
 }
 
@@ -653,19 +676,9 @@ struct FinishScratch {
   char* rows;          // a RowScratch for each warp
 };
 
-template <typename T>
-__device__ __forceinline__ Shared<T> shared_terms(const BeamSelectArgs& a, int seq, bool mix) {
-  Shared<T> sh{nullptr, nullptr, 0.0f};
-  if (mix) {
-    if (a.base != nullptr) sh.base = static_cast<const T*>(a.base) + (long long)seq * a.ld_base;
-    if (a.prior != nullptr) sh.prior = a.prior, sh.nbeta = -__ldg(a.beta);
-  }
-  return sh;
-}
-
 // The selection beam by beam: each one's `select` best candidates, then the best of those.
 // However many scores are equal, masked, or crowd together.
-template <typename T, bool MIX, bool VEC>
+template <typename T, bool VEC>
 __device__ __noinline__ void finish_exact(const BeamSelectArgs& a, const FinishScratch& f) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = blockDim.x >> 5;
   const int seq = blockIdx.x, n = a.select, total = a.beams * n;
@@ -673,7 +686,7 @@ __device__ __noinline__ void finish_exact(const BeamSelectArgs& a, const FinishS
   w.list = reinterpret_cast<unsigned long long*>(f.rows) + warp * kBeamListCap;
   w.quarters = reinterpret_cast<int*>(f.rows + n_warps * kBeamListCap * 8) + warp * kBeamListCap;
   w.count = reinterpret_cast<int*>(f.rows + n_warps * kBeamListCap * 12) + warp;
-  const Shared<T> sh = shared_terms<T>(a, seq, MIX);
+  const Shared<T> sh = shared_terms<T>(a, seq);
 #pragma unroll 1
   for (int k = warp; k < a.beams; k += n_warps) {
     const int row = seq * a.beams + k;
@@ -687,7 +700,7 @@ __device__ __noinline__ void finish_exact(const BeamSelectArgs& a, const FinishS
       }
       continue;
     }
-    const int c = row_best<T, MIX, VEC>(a, static_cast<const T*>(a.logits) + (long long)row * a.ld, sh,
+    const int c = row_best<T, VEC>(a, static_cast<const T*>(a.logits) + (long long)row * a.ld, sh,
                                         a.ws.group_top + (long long)row * a.groups, w);
     __syncwarp();
     for (int i = lane; i < c; i += 32) {
@@ -727,7 +740,7 @@ __device__ __noinline__ void finish_exact(const BeamSelectArgs& a, const FinishS
 // bound (about `select` of all beams together), and only they are read again, a warp each.
 // Where the bound says little (masked rows, many equal scores, more candidates than the list
 // holds) the CTA counts exactly, beam by beam.
-template <typename T, bool MIX, bool VEC>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(BeamSelectArgs a) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int n_found, n_quarters;
@@ -748,7 +761,7 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
   f.entries = reinterpret_cast<BeamEntry*>(rest + n_warps * kBeamRowScratch);
   f.score = reinterpret_cast<uint32_t*>(f.entries + a.beams * n);
   if (threadIdx.x == 0) n_found = n_quarters = 0;
-  const int blocks_per_seq = (a.beams + a.scan_rows - 1) / a.scan_rows;
+  const int run_blocks = (a.run_rows + a.scan_rows - 1) / a.scan_rows;
   pdl_wait();
 #pragma unroll 1
   for (int k = warp / split; k < a.beams; k += at_once) {
@@ -758,7 +771,7 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
     float2 st = make_float2(0.0f, cum);
     float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
     if (!done) {
-      const int unit = (seq * blocks_per_seq + k / a.scan_rows) * a.groups;
+      const int unit = (row / a.run_rows * run_blocks + row % a.run_rows / a.scan_rows) * a.groups;
       const int parts = a.share.cta(unit + a.groups - 1) - a.share.cta(unit) + 1;
       const float2* row_part = a.ws.part + (long long)row * a.parts;
       float2 p = __ldcg(row_part + min(lane, parts - 1));
@@ -855,14 +868,14 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
       }
     }
     __syncthreads();
-    const Shared<T> sh = shared_terms<T>(a, seq, MIX);
+    const Shared<T> sh = shared_terms<T>(a, seq);
     const int n_list = min(n_quarters, kBeamFinishCap);
 #pragma unroll 1
     for (int i = warp; i < n_list; i += n_warps) {
       const int k = f.quarters[i].x, q = f.quarters[i].y;
       const float2 st = f.stat[k];
       float2 x[2];
-      load_quarter<T, MIX, VEC>(a, static_cast<const T*>(a.logits) + (long long)(seq * a.beams + k) * a.ld, sh, q, lane, x);
+      load_quarter<T, VEC>(a, static_cast<const T*>(a.logits) + (long long)(seq * a.beams + k) * a.ld, sh, q, lane, x);
       if (row_score(fmax_nan(fmax3_nan(x[0].x, x[0].y, x[1].x), x[1].y), st) < bound) continue;
 #pragma unroll 1
       for (int j = 0; j < 4; ++j) {
@@ -879,13 +892,13 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
     const int row = seq * a.beams;
     const bool done = a.finished != nullptr && a.finished[row] != 0;
     if (warp == 0 && fabsf(f.stat[0].y) < __int_as_float(0x7f800000)) {
-      const Shared<T> sh = shared_terms<T>(a, seq, MIX);
+      const Shared<T> sh = shared_terms<T>(a, seq);
       const T* logits = static_cast<const T*>(a.logits) + (long long)row * a.ld;
       int c = n_found;
 #pragma unroll 1
       for (int v0 = 0; v0 < a.V && c < n; v0 += 32) {
         const int v = v0 + lane;
-        const bool masked = v < a.V && (done ? v != a.pad_token : mixed_logit<T, MIX>(logits, sh, v) == neg_inf());
+        const bool masked = v < a.V && (done ? v != a.pad_token : mixed_logit<T>(logits, sh, v) == neg_inf());
         const uint32_t take = __ballot_sync(kAllLanes, masked);
         // at most select + 31 candidates
         if (masked) f.list[c + __popc(take & ((1u << lane) - 1u))] = {((unsigned long long)none << 32) | 0xFFFFFFFFu,
@@ -898,7 +911,7 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
   }
   const int c = n_found;
   if (exact || n_quarters > kBeamFinishCap || c < n || c > kBeamFinishCap) {
-    finish_exact<T, MIX, VEC>(a, f);
+    finish_exact<T, VEC>(a, f);
     return;
   }
   for (int i = threadIdx.x; i < c; i += blockDim.x) {
@@ -918,22 +931,14 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
   }
 }
 
-BeamKernel beam_scan_kernel_for(bool bf16, bool mix, bool vec) {
-  static const BeamKernel kernels[8] = {
-      beam_scan_kernel<float, false, false>,         beam_scan_kernel<float, false, true>,
-      beam_scan_kernel<float, true, false>,          beam_scan_kernel<float, true, true>,
-      beam_scan_kernel<__nv_bfloat16, false, false>, beam_scan_kernel<__nv_bfloat16, false, true>,
-      beam_scan_kernel<__nv_bfloat16, true, false>,  beam_scan_kernel<__nv_bfloat16, true, true>};
-  return kernels[4 * bf16 + 2 * mix + vec];
+BeamKernel beam_scan_kernel_for(bool bf16, bool vec) {
+  if (bf16) return vec ? beam_scan_kernel<__nv_bfloat16, true> : beam_scan_kernel<__nv_bfloat16, false>;
+  return vec ? beam_scan_kernel<float, true> : beam_scan_kernel<float, false>;
 }
 
-BeamKernel beam_finish_kernel_for(bool bf16, bool mix, bool vec) {
-  static const BeamKernel kernels[8] = {
-      beam_finish_kernel<float, false, false>,         beam_finish_kernel<float, false, true>,
-      beam_finish_kernel<float, true, false>,          beam_finish_kernel<float, true, true>,
-      beam_finish_kernel<__nv_bfloat16, false, false>, beam_finish_kernel<__nv_bfloat16, false, true>,
-      beam_finish_kernel<__nv_bfloat16, true, false>,  beam_finish_kernel<__nv_bfloat16, true, true>};
-  return kernels[4 * bf16 + 2 * mix + vec];
+BeamKernel beam_finish_kernel_for(bool bf16, bool vec) {
+  if (bf16) return vec ? beam_finish_kernel<__nv_bfloat16, true> : beam_finish_kernel<__nv_bfloat16, false>;
+  return vec ? beam_finish_kernel<float, true> : beam_finish_kernel<float, false>;
 }
 
 // --------------------------------------------------------------------------------

@@ -9,7 +9,8 @@ namespace dels {
 constexpr int kBeamMax = 64;         // beams of a sequence, read or selected
 constexpr int kBeamGroup = 512;      // logits of a group, the unit a warp scans at a time
 constexpr int kBeamScanWarps = 4;    // most warps of a scanning CTA
-constexpr int kBeamScanRows = 8;     // most rows a scanning CTA takes through the logits they share
+constexpr int kBeamScanRows = 8;     // most rows a scanning CTA takes together
+constexpr int kBeamScanCtas = 6;     // most scanning CTAs of an SM
 constexpr int kBeamFinishWarps = 16; // most warps of a sequence's finishing CTA
 constexpr int kBeamFinishCap = 256;  // quarter groups or candidates it lists before it counts exactly
 constexpr int kBeamListCap = 192;    // counting exactly: quarter groups or logits a warp lists
@@ -52,7 +53,8 @@ struct BeamSelectArgs {
   int pad_token;
   int n_seq, beams, select, V;
   int groups, parts;
-  int scan_rows;             // rows that are scanned together (a block of rows)
+  int run_rows;              // rows that blocks are cut from: a sequence's where they share logits, else all
+  int scan_rows;             // rows of a block, scanned together
   int scan_ctas;
   ScanShare share;
   int finish_split;          // warps of the finishing CTA that share a beam
@@ -65,19 +67,19 @@ struct BeamSelectArgs {
   BeamScratch ws;
 };
 
-// Warps that scan a group together, two rows (MIX) each, and teams of them in a CTA.
+// Warps that scan a group together, two rows each, and teams of them in a CTA.
 __host__ __device__ __forceinline__ int scan_pairs(int rows) { return (rows + 1) / 2; }
 __host__ __device__ __forceinline__ int scan_teams(int rows) { return kBeamScanWarps / scan_pairs(rows); }
 
 // The scan's staging rings, one for each team: groups in flight.
-constexpr int beam_scan_depth(int elem, bool mix) { return mix ? (elem == 2 ? 3 : 2) : 6; }
+constexpr int beam_scan_depth(int elem) { return elem == 2 ? 3 : 2; }
 // Bytes of a slot: `rows` rows of a group, and the draft logits and prior they share.
-constexpr int beam_slot_bytes(int rows, int elem, bool mix) {
-  return rows * kBeamGroup * elem + (mix ? kBeamGroup * (elem + 4) : 0);
+constexpr int beam_slot_bytes(int rows, int elem, bool shared) {
+  return rows * kBeamGroup * elem + (shared ? kBeamGroup * (elem + 4) : 0);
 }
 // Dynamic shared memory of beam_scan_kernel with VEC.
-inline int beam_scan_smem(int rows, int elem, bool mix) {
-  return scan_teams(rows) * beam_scan_depth(elem, mix) * beam_slot_bytes(rows, elem, mix);
+inline int beam_scan_smem(int rows, int elem, bool shared) {
+  return scan_teams(rows) * beam_scan_depth(elem) * beam_slot_bytes(rows, elem, shared);
 }
 constexpr int kBeamScanSmemMax = 65536;  // two rows of fp32: 4 teams x 2 slots x 8 KB
 
@@ -88,11 +90,10 @@ constexpr int beam_finish_smem(int beams, int select, int warps, int values) {
   return (beams * 8 + 15) / 16 * 16 + (listing > exact ? listing : exact);
 }
 
-// The kernels for bf16 or fp32 logits, with shared terms (mix) or without, and with 16-byte
-// loads (vec) or without.
+// The kernels for bf16 or fp32 logits, with 16-byte loads (vec) or without.
 using BeamKernel = void (*)(BeamSelectArgs);
-BeamKernel beam_scan_kernel_for(bool bf16, bool mix, bool vec);
-BeamKernel beam_finish_kernel_for(bool bf16, bool mix, bool vec);
+BeamKernel beam_scan_kernel_for(bool bf16, bool vec);
+BeamKernel beam_finish_kernel_for(bool bf16, bool vec);
 
 // One state of the beams: rows x outer x inner contiguous bytes.
 struct BeamState {
