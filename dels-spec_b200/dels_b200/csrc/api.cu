@@ -288,7 +288,8 @@ int init_device(int dev) {
     SET(gru_gates_kernel, 0);
     SET(gru_finalize_kernel, 0);
     SET(wait_selftest_kernel, 0);
-    SET_SHARED(beam_reorder_kernel, 0);
+    SET_SHARED(beam_reorder_kernel_many(), 0);
+    SET_SHARED(beam_reorder_kernel_few(), 0);
     for (int i = 0; i < 4; ++i) {
       const bool bf16 = (i & 2) != 0, vec = (i & 1) != 0;
       SET_SHARED(beam_scan_kernel_for(bf16, vec), vec ? kBeamScanSmemMax : 0);
@@ -1707,28 +1708,28 @@ int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const voi
   return launch_beam_select(a, dtype == DELS_DTYPE_BF16, shared, vec, reinterpret_cast<cudaStream_t>(stream));
 }
 
-int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t* parents, int n_seq, int beams,
+int dels_beam_reorder(const dels_beam_state* states_in, int n_states, const int32_t* parents, int n_seq, int beams,
                       int select, int32_t* status, void* stream) {
   int rc;
   if (n_seq < 0 || n_states < 0) return fail(DELS_ERR_INVALID_ARG, "bad counts n_seq=%d n_states=%d", n_seq, n_states);
   if (beams < 1 || beams > kBeamMax || select < 1 || select > kBeamMax)
     return fail(DELS_ERR_INVALID_ARG, "beams and select must be in 1..%d (got %d, %d)", kBeamMax, beams, select);
-  if (n_states > 0 && (states == nullptr || (parents == nullptr && n_seq > 0)))
+  if (n_states > 0 && (states_in == nullptr || (parents == nullptr && n_seq > 0)))
     return fail(DELS_ERR_INVALID_ARG, "NULL argument");
   for (int i = 0; i < n_states; ++i)
-    if ((rc = check_beam_state(states[i], i, n_seq, beams, select)) != DELS_OK) return rc;
+    if ((rc = check_beam_state(states_in[i], i, n_seq, beams, select)) != DELS_OK) return rc;
   DeviceState* ds = nullptr;
   if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
   if (n_seq == 0) return DELS_OK;
   // the widest piece of a row that all beams' copies of it leave room for in shared memory
   const int room = (kBeamReorderSmem / beams - 32) / 128 * 128;
   for (int first = 0; first < n_states; first += kBeamStatesPerLaunch) {
-    BeamReorderArgs a;
-    std::memset(&a, 0, sizeof(a));
+    BeamReorderArgs a = {parents, status, 0, 0, n_seq, beams, select};
+    BeamStates<kBeamStatesPerLaunch> states;
     for (int i = first; i < n_states && i < first + kBeamStatesPerLaunch; ++i) {
-      const dels_beam_state& d = states[i];
+      const dels_beam_state& d = states_in[i];
       if (d.outer == 0 || d.inner_bytes == 0) continue;
-      BeamState& s = a.st[a.n_states++];
+      BeamState& s = states.st[a.n_states++];
       s.src = static_cast<const char*>(d.src);
       s.dst = static_cast<char*>(d.dst);
       s.src_row = d.src_row_stride;
@@ -1743,15 +1744,18 @@ int dels_beam_reorder(const dels_beam_state* states, int n_states, const int32_t
       a.tiles += (long long)n_seq * s.outer * s.chunks;
     }
     if (a.tiles == 0) continue;
-    a.parents = parents;
-    a.n_seq = n_seq;
-    a.beams = beams;
-    a.select = select;
-    a.status = status;
     const long long most = (long long)kBeamReorderCtas * ds->sm_count;
-    DELS_CHECK_PDL("beam_reorder_kernel launch", launch_pdl(beam_reorder_kernel,
-        dim3((unsigned)(a.tiles < most ? a.tiles : most)), dim3(kBeamThreads), 0,
-        reinterpret_cast<cudaStream_t>(stream), a));
+    const dim3 grid((unsigned)(a.tiles < most ? a.tiles : most));
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (a.n_states <= kBeamFewStates) {
+      BeamStates<kBeamFewStates> few;
+      for (int i = 0; i < a.n_states; ++i) few.st[i] = states.st[i];
+      DELS_CHECK_PDL("beam_reorder_kernel launch",
+                     launch_pdl(beam_reorder_kernel_few(), grid, dim3(kBeamThreads), 0, st, a, few));
+    } else {
+      DELS_CHECK_PDL("beam_reorder_kernel launch",
+                     launch_pdl(beam_reorder_kernel_many(), grid, dim3(kBeamThreads), 0, st, a, states));
+    }
   }
   return DELS_OK;
 }

@@ -999,7 +999,9 @@ __device__ __forceinline__ void write_row(char* dst, const char* from, int bytes
 
 }  // namespace
 
-__global__ void __launch_bounds__(kBeamThreads) beam_reorder_kernel(const __grid_constant__ BeamReorderArgs a) {
+template <int N>
+__global__ void __launch_bounds__(kBeamThreads)
+    beam_reorder_kernel(const BeamReorderArgs a, const __grid_constant__ BeamStates<N> states) {
   __shared__ __align__(16) char stage[kBeamReorderSmem];
   __shared__ int parent[kBeamMax];
   __shared__ unsigned long long used;
@@ -1009,8 +1011,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_reorder_kernel(const __grid
   pdl_wait();
   for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     int k = 0;
-    while (k + 1 < a.n_states && tile >= a.st[k + 1].tile0) ++k;
-    const BeamState& st = a.st[k];
+    while (k + 1 < a.n_states && tile >= states.st[k + 1].tile0) ++k;
+    const BeamState& st = states.st[k];
     const long long local = tile - st.tile0;
     const int c = (int)(local % st.chunks);
     const long long rest = local / st.chunks;
@@ -1055,5 +1057,8 @@ __global__ void __launch_bounds__(kBeamThreads) beam_reorder_kernel(const __grid
     }
   }
 }
+
+BeamReorderKernel beam_reorder_kernel_many() { return beam_reorder_kernel<kBeamStatesPerLaunch>; }
+BeamReorderFewKernel beam_reorder_kernel_few() { return beam_reorder_kernel<kBeamFewStates>; }
 
 }  // namespace dels

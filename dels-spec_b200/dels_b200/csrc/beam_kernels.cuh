@@ -107,22 +107,31 @@ struct BeamState {
   long long tile0;   // first tile of this state
 };
 
+// States of a launch; a few are passed in a shorter list (copying 2 KB of arguments for each
+// launch costs the host about as much as launching).
 constexpr int kBeamStatesPerLaunch = 32;
+constexpr int kBeamFewStates = 4;
 constexpr int kBeamThreads = 256;
 
 struct BeamReorderArgs {
-  BeamState st[kBeamStatesPerLaunch];
-  int n_states;
   const int* parents;  // [n_seq, select]
-  int n_seq, beams, select;
   int* status;         // or null
   long long tiles;
+  int n_states;
+  int n_seq, beams, select;
+};
+template <int N>
+struct BeamStates {
+  BeamState st[N];
 };
 
 // A tile's stage: each beam's piece, up to 15 bytes before it and a word after.
 constexpr int kBeamReorderSmem = 33792;
 constexpr int kBeamReorderCtas = 5;  // an SM holds: 617 MB of a cache in 97 us; a sixth would wait its turn (126 us)
 
-__global__ void beam_reorder_kernel(const __grid_constant__ BeamReorderArgs a);
+using BeamReorderKernel = void (*)(BeamReorderArgs, BeamStates<kBeamStatesPerLaunch>);
+using BeamReorderFewKernel = void (*)(BeamReorderArgs, BeamStates<kBeamFewStates>);
+BeamReorderKernel beam_reorder_kernel_many();
+BeamReorderFewKernel beam_reorder_kernel_few();
 
 }  // namespace dels

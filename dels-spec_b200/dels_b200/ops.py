@@ -1127,25 +1127,27 @@ def beam_reorder(
     overlap otherwise.  A parent outside 0..beams-1 leaves its child's row as it was and
     stores an error code in ``status`` (int32 [1], zero before)."""
     _require_cuda("parents", parents, torch.int32, 2)
-    dev = parents.device
+    if not parents.is_contiguous():
+        raise ValueError(f"parents must be contiguous (stride {parents.stride()})")
+    dev, index = parents.device, parents.get_device()
     n_seq, n = parents.shape
-    _require_dense("parents", parents, torch.int32, (n_seq, n), dev)
     if status is not None:
         _require_dense("status", status, torch.int32, (1,), dev)
-    rows = n_seq * int(beams)
+    rows, out_rows = n_seq * int(beams), n_seq * n
     if out is None:
-        out = [torch.empty((n_seq * n, *t.shape[1:]), dtype=t.dtype, device=dev) for t in states]
+        out = [torch.empty((out_rows, *t.shape[1:]), dtype=t.dtype, device=dev) for t in states]
     if len(out) != len(states):
         raise ValueError(f"{len(states)} states, but {len(out)} outputs")
     table: list[int] = []
     for i, (src, dst) in enumerate(zip(states, out)):
-        if src.device != dev or dst.device != dev:
+        have, want = src.shape, dst.shape
+        if src.get_device() != index or dst.get_device() != index:
             raise ValueError(f"state {i}: {src.device} -> {dst.device}, but parents are on {dev}")
-        if src.dim() < 1 or src.shape[0] != rows or dst.dtype != src.dtype or dst.shape[0] != n_seq * n \
-                or dst.shape[1:] != src.shape[1:]:
-            raise ValueError(f"state {i}: {src.dtype} {tuple(src.shape)} -> {dst.dtype} {tuple(dst.shape)} does not "
-                             f"match {n_seq} sequences of {beams} -> {n} beams")
-        table.extend(_beam_state(i, src, dst))
+        if not have or not want or have[0] != rows or want[0] != out_rows or have[1:] != want[1:] \
+                or src.dtype != dst.dtype:
+            raise ValueError(f"state {i}: {src.dtype} {tuple(have)} -> {dst.dtype} {tuple(want)} does not match "
+                             f"{n_seq} sequences of {beams} -> {n} beams")
+        table += _beam_state(i, src, dst)
     _lib.call("dels_beam_reorder", _int64_array(len(table))(*table), len(states), _addr(parents), n_seq, int(beams), n,
               _addr(status), _raw_stream(dev))
     return out
