@@ -877,6 +877,7 @@ int launch_i8_tn(const void* xq, long long ld_x, const void* wq, long long ld_w,
   if ((rc = make_map_i8(&mw, wq, K, a.n_out, ld_w, a.box)) != DELS_OK) return rc;
   if ((rc = make_map_i8(&mx, xq, K, a.rows, ld_x, TN)) != DELS_OK) return rc;
   const long long units = (long long)a.n_tiles * a.m_tiles;
+  if (units > INT32_MAX) return fail(DELS_ERR_UNSUPPORTED, "product of %d rows and %d channels is too large", a.rows, a.n_out);
   DELS_CHECK_PDL("i8_gemm_kernel launch",
                  launch_pdl(i8_gemm_kernel<TN, OutT>, dim3((unsigned)(units < sm_count ? units : sm_count)),
                             dim3(kI8Threads), I8Config<TN>::kFixedBytes + a.stages * I8Config<TN>::slot_bytes(box), st,
@@ -896,6 +897,7 @@ int launch_i8_pair(const void* xq, long long ld_x, const void* wq, long long ld_
   a.bn = cdiv(cdiv(a.rows, a.m_tiles), 32) * 32;
   a.tail = a.bn % 128 == 0 ? 4 : (a.bn % 64 == 0 ? 2 : 1);  // split tiles are multiples of 32, too
   const long long tiles = (long long)a.m_tiles * a.n_tiles;
+  if (tiles > INT32_MAX / 4) return fail(DELS_ERR_UNSUPPORTED, "product of %d rows and %d channels is too large", a.rows, a.n_out);
   const long long want = tiles < max_pairs ? tiles * a.tail : tiles;
   CUtensorMap mw, mx, mxt;
   if ((rc = make_map_i8(&mw, wq, K, a.n_out, ld_w, kBM)) != DELS_OK) return rc;

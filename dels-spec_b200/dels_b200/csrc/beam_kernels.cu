@@ -21,6 +21,9 @@
 // Both kernels are short loops on purpose: a step of one sequence runs each instruction a
 // few times only, and then fetching code costs more than executing it (unrolled over four
 // rows, the scan of 4 x 151936 logits took 23 us for 810 instructions a warp).
+//
+// A kernel here may start before the one that makes its inputs has ended (programmatic
+// dependent launch), so nothing is read through the read-only path.
 #include "beam_kernels.cuh"
 
 namespace dels {
@@ -95,7 +98,7 @@ template <>
 struct Raw4<float> {
   float4 w;
   __device__ __forceinline__ void load(const float* p) {
-    asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];"
                  : "=f"(w.x), "=f"(w.y), "=f"(w.z), "=f"(w.w)
                  : "l"(p));
   }
@@ -105,7 +108,7 @@ template <>
 struct Raw4<__nv_bfloat16> {
   uint2 w;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) {
-    asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "l"(p));
+    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "l"(p));
   }
   __device__ __forceinline__ void unpack(float2 (&x)[2]) const {
     x[0] = make_float2(bf16_lo(w.x), bf16_hi(w.x)), x[1] = make_float2(bf16_lo(w.y), bf16_hi(w.y));
@@ -148,7 +151,7 @@ template <typename T>
 __device__ __forceinline__ Shared<T> shared_terms(const BeamSelectArgs& a, int seq) {
   Shared<T> sh{nullptr, nullptr, 0.0f};
   if (a.base != nullptr) sh.base = static_cast<const T*>(a.base) + (long long)seq * a.ld_base;
-  if (a.prior != nullptr) sh.prior = a.prior, sh.nbeta = -__ldg(a.beta);
+  if (a.prior != nullptr) sh.prior = a.prior, sh.nbeta = -*a.beta;
   return sh;
 }
 
@@ -157,7 +160,7 @@ template <typename T>
 __device__ __forceinline__ float mixed_logit(const T* row, const Shared<T>& sh, int v) {
   float x = to_f32(row[v]);
   if (sh.base != nullptr) x = __fadd_rn(to_f32(sh.base[v]), x);
-  if (sh.prior != nullptr) x = __fadd_rn(x, __fmul_rn(sh.nbeta, __ldg(sh.prior + v)));
+  if (sh.prior != nullptr) x = __fadd_rn(x, __fmul_rn(sh.nbeta, sh.prior[v]));
   return x;
 }
 
@@ -180,7 +183,7 @@ __device__ __forceinline__ void load_single(const T* const (&row)[2], const Shar
     }
     if (sh.prior != nullptr) {
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) p[j] = __ldg(sh.prior + v0 + 32 * j + lane);
+      for (int j = 0; j < kPer; ++j) p[j] = sh.prior[v0 + 32 * j + lane];
     }
 #pragma unroll
     for (int i = 0; i < kPer / 2; ++i)
@@ -489,7 +492,7 @@ __device__ __noinline__ void row_best_exact(const BeamSelectArgs& a, const T* lo
   const int n_groups = min(a.select, a.groups);
   warp_top(a.groups, n_groups,
            [&](int i) {
-             const float4 t = __ldg(tops + i);
+             const float4 t = __ldcg(tops + i);
              return ordered_u32(fmax_nan(fmax3_nan(t.x, t.y, t.z), t.w));
            },
            [&](int slot, int i, uint32_t) { w.quarters[slot] = i; });
@@ -584,7 +587,7 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
   if (!few) {
 #pragma unroll 5
     for (int i = lane; i < a.groups; i += 32) {
-      const float4 t = __ldg(tops + i);
+      const float4 t = __ldcg(tops + i);
       top[0] = max(top[0], ordered_u32(t.x)), top[1] = max(top[1], ordered_u32(t.y));
       top[2] = max(top[2], ordered_u32(t.z)), top[3] = max(top[3], ordered_u32(t.w));
     }
@@ -607,7 +610,7 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
     __syncwarp();
 #pragma unroll 1
     for (int i = lane; i < a.groups; i += 32) {
-      const float4 t = __ldg(tops + i);
+      const float4 t = __ldcg(tops + i);
       // NaN counts as above every bound
       uint32_t reach = (t.x < floor ? 0u : 1u) | (t.y < floor ? 0u : 2u) | (t.z < floor ? 0u : 4u) | (t.w < floor ? 0u : 8u);
 #pragma unroll 1
@@ -767,7 +770,7 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
   for (int k = warp / split; k < a.beams; k += at_once) {
     const int row = seq * a.beams + k;
     const bool done = a.finished != nullptr && a.finished[row] != 0;
-    const float cum = __ldg(a.cum + row);
+    const float cum = __ldcg(a.cum + row);
     float2 st = make_float2(0.0f, cum);
     float top[4] = {neg_inf(), neg_inf(), neg_inf(), neg_inf()};
     if (!done) {
@@ -778,7 +781,7 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
       const float4* tops = a.ws.group_top + (long long)row * a.groups;
 #pragma unroll 5
       for (int i = part * 32 + lane; i < a.groups; i += 32 * split) {
-        const float4 t = __ldg(tops + i);
+        const float4 t = __ldcg(tops + i);
         top[0] = fmax_nan(top[0], t.x), top[1] = fmax_nan(top[1], t.y);
         top[2] = fmax_nan(top[2], t.z), top[3] = fmax_nan(top[3], t.w);
       }
@@ -856,7 +859,7 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
       const float4* tops = a.ws.group_top + (long long)row * a.groups;
 #pragma unroll 5
       for (int i = part * 32 + lane; i < a.groups; i += 32 * split) {
-        const float4 t = __ldg(tops + i);
+        const float4 t = __ldcg(tops + i);
         // (a NaN reaches every bound)
         if (row_score(fmax_nan(fmax3_nan(t.x, t.y, t.z), t.w), st) < bound) continue;
 #pragma unroll 1

@@ -289,11 +289,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       const int valid = min(TN, args.rows - m0);
       if (m_tile != scale_m) {
         __syncwarp();
-        for (int j = lane; j < TN; j += 32) scale[j] = m0 + j < args.rows ? __ldg(args.sx + m0 + j) : 0.0f;
+        for (int j = lane; j < TN; j += 32) scale[j] = m0 + j < args.rows ? args.sx[m0 + j] : 0.0f;
         __syncwarp();
         scale_m = m_tile;
       }
-      const float sw = channel_ok ? __ldg(args.sw + n) : 0.0f;
+      const float sw = channel_ok ? args.sw[n] : 0.0f;
       float bias = 0.0f;
       if (channel_ok && bias_v != nullptr) {
         if constexpr (sizeof(OutT) == 2)
@@ -563,11 +563,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
       const int valid = min(rows, args.rows - m0);  // may be <= 0 in a split tile
       if (m0 != scale_m) {
         __syncwarp();
-        for (int j = lane; j < rows; j += 32) scale[j] = m0 + j < args.rows ? __ldg(args.sx + m0 + j) : 0.0f;
+        for (int j = lane; j < rows; j += 32) scale[j] = m0 + j < args.rows ? args.sx[m0 + j] : 0.0f;
         __syncwarp();
         scale_m = m0;
       }
-      const float sw = channel_ok ? __ldg(args.sw + n) : 0.0f;
+      const float sw = channel_ok ? args.sw[n] : 0.0f;
       float bias = 0.0f;
       if (channel_ok && bias_v != nullptr) {
         if constexpr (sizeof(OutT) == 2)

@@ -12,12 +12,12 @@ namespace dels {
 namespace {
 
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-  const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  const float4 b = *(reinterpret_cast<const float4*>(p) + 1);
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
   x[0] = bf16_lo(w.x), x[1] = bf16_hi(w.x), x[2] = bf16_lo(w.y), x[3] = bf16_hi(w.y);
   x[4] = bf16_lo(w.z), x[5] = bf16_hi(w.z), x[6] = bf16_lo(w.w), x[7] = bf16_hi(w.w);
 }
@@ -108,7 +108,7 @@ namespace {
 
 __device__ __forceinline__ uint4 load_weights(const int8_t* p) {
   uint4 w;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                : "l"(p));
   return w;
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kI8GemvThreads, kI8GemvCtas) i8_gemv_kernel(I8
     if constexpr (sizeof(T) == 1) {
       const int8_t* src = static_cast<const int8_t*>(a.x) + (long long)r * a.ld_x;
       for (int c = threadIdx.x; c < whole; c += kI8GemvThreads)
-        reinterpret_cast<uint4*>(dst)[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+        reinterpret_cast<uint4*>(dst)[c] = reinterpret_cast<const uint4*>(src)[c];
       for (int k = 16 * whole + threadIdx.x; k < a.K; k += kI8GemvThreads) dst[k] = src[k];
       if (threadIdx.x == 0) scale[r] = a.sx[r];
     } else {
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kI8GemvThreads, kI8GemvCtas) i8_gemv_kernel(I8
       mine = lane == r ? total : mine;
     }
     if (lane < a.rows) {
-      float y = __int2float_rn(mine) * scale[lane] * __ldg(a.sw + n);
+      float y = __int2float_rn(mine) * scale[lane] * a.sw[n];
       if (a.bias != nullptr) y += to_f32(static_cast<const OutT*>(a.bias)[n]);
       OutT* out = static_cast<OutT*>(a.out) + (long long)lane * a.ld_out + n;
       if constexpr (sizeof(OutT) == 2)
