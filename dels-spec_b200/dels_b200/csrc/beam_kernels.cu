@@ -276,6 +276,7 @@ __global__ void __launch_bounds__(32 * kBeamScanWarps, kBeamScanCtas) beam_scan_
   if (threadIdx.x == 0) aborted = 0;
   __syncthreads();
   pdl_wait();
+  pdl_trigger();
   int slot = 0, fill_slot = 0;
   uint32_t parity = 0, fill_parity = 0;
 #pragma unroll 1
@@ -766,6 +767,7 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
   if (threadIdx.x == 0) n_found = n_quarters = 0;
   const int run_blocks = (a.run_rows + a.scan_rows - 1) / a.scan_rows;
   pdl_wait();
+  pdl_trigger();
 #pragma unroll 1
   for (int k = warp / split; k < a.beams; k += at_once) {
     const int row = seq * a.beams + k;
@@ -1012,6 +1014,7 @@ __global__ void __launch_bounds__(kBeamThreads)
   constexpr int kWarps = kBeamThreads / 32;
   const int row_room = kBeamReorderSmem / a.beams & ~15;
   pdl_wait();
+  pdl_trigger();
   for (long long tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     int k = 0;
     while (k + 1 < a.n_states && tile >= states.st[k + 1].tile0) ++k;
