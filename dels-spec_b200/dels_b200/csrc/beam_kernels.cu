@@ -663,6 +663,17 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
 // Score of a logit in a row with (m, cum - log S) = st.
 __device__ __forceinline__ float row_score(float x, float2 st) { return x == neg_inf() ? neg_inf() : (x - st.x) + st.y; }
 
+// Group maxima of a lane at once, before the first of them is used: those of i, i + step, ...;
+// -inf past the end (a maximum offered twice would raise the bound above too many others).
+constexpr int kFinishLoads = 5;
+__device__ __forceinline__ void load_tops(const float4* tops, int i, int step, int groups, float4 (&t)[kFinishLoads]) {
+#pragma unroll
+  for (int u = 0; u < kFinishLoads; ++u) t[u] = __ldcg(tops + min(i + u * step, groups - 1));
+#pragma unroll
+  for (int u = 1; u < kFinishLoads; ++u)
+    if (i + u * step >= groups) t[u] = make_float4(neg_inf(), neg_inf(), neg_inf(), neg_inf());
+}
+
 // A candidate: (score, beam) and (x, token), both in the order in which larger is better.
 struct Candidate {
   unsigned long long rank, within;
@@ -781,11 +792,15 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
       const float2* row_part = a.ws.part + (long long)row * a.parts;
       float2 p = __ldcg(row_part + min(lane, parts - 1));
       const float4* tops = a.ws.group_top + (long long)row * a.groups;
-#pragma unroll 5
-      for (int i = part * 32 + lane; i < a.groups; i += 32 * split) {
-        const float4 t = __ldcg(tops + i);
-        top[0] = fmax_nan(top[0], t.x), top[1] = fmax_nan(top[1], t.y);
-        top[2] = fmax_nan(top[2], t.z), top[3] = fmax_nan(top[3], t.w);
+#pragma unroll 1
+      for (int i = part * 32 + lane; i < a.groups; i += kFinishLoads * 32 * split) {
+        float4 t[kFinishLoads];
+        load_tops(tops, i, 32 * split, a.groups, t);
+#pragma unroll
+        for (int u = 0; u < kFinishLoads; ++u) {
+          top[0] = fmax_nan(top[0], t[u].x), top[1] = fmax_nan(top[1], t[u].y);
+          top[2] = fmax_nan(top[2], t[u].z), top[3] = fmax_nan(top[3], t[u].w);
+        }
       }
       if (lane >= parts) p = make_float2(neg_inf(), 0.0f);
 #pragma unroll 1
@@ -859,16 +874,21 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
       const uint32_t* value = f.value + ((k * split + part) * 32 + lane) * per_lane;
       if (value[0] < key && (per_lane == 1 || max(max(value[1], value[2]), value[3]) < key)) continue;
       const float4* tops = a.ws.group_top + (long long)row * a.groups;
-#pragma unroll 5
-      for (int i = part * 32 + lane; i < a.groups; i += 32 * split) {
-        const float4 t = __ldcg(tops + i);
-        // (a NaN reaches every bound)
-        if (row_score(fmax_nan(fmax3_nan(t.x, t.y, t.z), t.w), st) < bound) continue;
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          if (row_score(q & 2 ? (q & 1 ? t.w : t.z) : (q & 1 ? t.y : t.x), st) < bound) continue;
-          const int slot = atomicAdd(&n_quarters, 1);
-          if (slot < kBeamFinishCap) f.quarters[slot] = make_int2(k, 4 * i + q);
+      for (int i = part * 32 + lane; i < a.groups; i += kFinishLoads * 32 * split) {
+        float4 t[kFinishLoads];
+        load_tops(tops, i, 32 * split, a.groups, t);
+#pragma unroll
+        for (int u = 0; u < kFinishLoads; ++u) {
+          const int g = i + u * 32 * split;
+          // (a NaN reaches every bound)
+          if (row_score(fmax_nan(fmax3_nan(t[u].x, t[u].y, t[u].z), t[u].w), st) < bound) continue;
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            if (row_score(q & 2 ? (q & 1 ? t[u].w : t[u].z) : (q & 1 ? t[u].y : t[u].x), st) < bound) continue;
+            const int slot = atomicAdd(&n_quarters, 1);
+            if (slot < kBeamFinishCap) f.quarters[slot] = make_int2(k, 4 * g + q);
+          }
         }
       }
     }
