@@ -878,6 +878,14 @@ def _require_dense(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple,
                          f"(got {t.dtype} {tuple(t.shape)} on {t.device}, stride {t.stride()})")
 
 
+def _leading(name: str, t: torch.Tensor) -> int:
+    """_row_major() of a tensor that is known to have two dimensions."""
+    (rows, cols), (ld, step) = t.shape, t.stride()
+    if step != 1 and cols > 1 and rows > 0:
+        raise ValueError(f"{name} must have contiguous rows (stride {(ld, step)})")
+    return ld if rows > 1 and cols > 0 else max(ld, cols, 1)
+
+
 # A draft step calls these operators on small tensors, where the host's part of a call is what
 # counts: addresses go to ctypes as plain integers, sizes of workspaces are asked for once.
 def _addr(t: torch.Tensor | None) -> int | None:
@@ -919,7 +927,7 @@ def quantize_rows_i8(
         scale = torch.empty(rows, dtype=torch.float32, device=dev)
     else:
         _require_dense("scale", scale, torch.float32, (rows,), dev)
-    _lib.call("dels_quantize_rows_i8", _addr(x), code, _row_major("x", x), rows, K, _addr(q), _row_major("q", q),
+    _lib.call("dels_quantize_rows_i8", _addr(x), code, _leading("x", x), rows, K, _addr(q), _leading("q", q),
               _addr(scale), _raw_stream(dev))
     return q, scale
 
@@ -964,8 +972,8 @@ def linear_i8(
     N, out = _i8_operands(rows, K, dev, wq, w_scale, bias, out, out_dtype)
     stream = _raw_stream(dev)
     ws = _stream_workspace(_lib.DELS_WS_HEADER_BYTES, dev, stream) if ws is None else ws
-    _lib.call("dels_linear_i8", _addr(xq), _row_major("xq", xq), _addr(x_scale), _addr(wq), _row_major("wq", wq),
-              _addr(w_scale), _addr(bias), rows, K, N, _addr(out), _FLOATS[out.dtype], _row_major("out", out), ws.ptr,
+    _lib.call("dels_linear_i8", _addr(xq), _leading("xq", xq), _addr(x_scale), _addr(wq), _leading("wq", wq),
+              _addr(w_scale), _addr(bias), rows, K, N, _addr(out), _FLOATS[out.dtype], _leading("out", out), ws.ptr,
               ws.nbytes, stream)
     return out
 
@@ -995,8 +1003,8 @@ def linear_w8a8(
     need = linear_w8a8_workspace_bytes(rows, K)
     stream = _raw_stream(dev)
     ws = _stream_workspace(need, dev, stream) if ws is None else ws.ensure(need)
-    _lib.call("dels_linear_w8a8", _addr(x), code, _row_major("x", x), _addr(wq), _row_major("wq", wq), _addr(w_scale),
-              _addr(bias), rows, K, N, _addr(out), _FLOATS[out.dtype], _row_major("out", out), ws.ptr, ws.nbytes,
+    _lib.call("dels_linear_w8a8", _addr(x), code, _leading("x", x), _addr(wq), _leading("wq", wq), _addr(w_scale),
+              _addr(bias), rows, K, N, _addr(out), _FLOATS[out.dtype], _leading("out", out), ws.ptr, ws.nbytes,
               stream)
     return out
 
@@ -1067,8 +1075,8 @@ def beam_select(
     stream = _raw_stream(dev)
     ws = _stream_workspace(need, dev, stream) if ws is None else ws.ensure(need)
     _lib.call(
-        "dels_beam_select", _addr(logits), code, _row_major("logits", logits), _addr(base),
-        0 if base is None else _row_major("base", base), _addr(prior), _addr(beta), _addr(scores), _addr(finished),
+        "dels_beam_select", _addr(logits), code, _leading("logits", logits), _addr(base),
+        0 if base is None else _leading("base", base), _addr(prior), _addr(beta), _addr(scores), _addr(finished),
         int(pad_token), n_seq, beams, n, V, _addr(out.parents), _addr(out.tokens), _addr(out.scores), ws.ptr,
         ws.nbytes, stream,
     )
@@ -1086,12 +1094,12 @@ def _int64_array(n: int):
 
 def _beam_state(i: int, src: torch.Tensor, dst: torch.Tensor) -> tuple:
     """The dels_beam_state of one (src, dst) pair: rows of ``outer`` runs of contiguous bytes."""
-    item = src.element_size()
+    shape = src.shape
     if src.is_contiguous() and dst.is_contiguous():
         # (by its size: the stride of a dimension of one row may be anything)
-        row = src.numel() // src.shape[0] * item if src.shape[0] else 0
+        row = src.nbytes // shape[0] if shape[0] else 0
         return src.data_ptr(), dst.data_ptr(), row, row, 0, 0, 1, row
-    shape, ss, ds = src.shape, src.stride(), dst.stride()
+    item, ss, ds = src.element_size(), src.stride(), dst.stride()
     inner, k = 1, src.dim() - 1
     while k >= 1 and (shape[k] == 1 or (ss[k] == inner and ds[k] == inner)):
         inner *= shape[k]
@@ -1143,7 +1151,7 @@ def beam_reorder(
         have, want = src.shape, dst.shape
         if src.get_device() != index or dst.get_device() != index:
             raise ValueError(f"state {i}: {src.device} -> {dst.device}, but parents are on {dev}")
-        if not have or not want or have[0] != rows or want[0] != out_rows or have[1:] != want[1:] \
+        if not have or have[0] != rows or want != (have if n == beams else (out_rows, *have[1:])) \
                 or src.dtype != dst.dtype:
             raise ValueError(f"state {i}: {src.dtype} {tuple(have)} -> {dst.dtype} {tuple(want)} does not match "
                              f"{n_seq} sequences of {beams} -> {n} beams")
