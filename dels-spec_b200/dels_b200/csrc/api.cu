@@ -863,6 +863,28 @@ I8Shape plan_i8(int rows, int n_out, int sm_count) {
   return best;
 }
 
+// The tiles of i8_pair_kernel: 256 channels x bn rows, those of a partial last wave split along
+// the rows as far as their parts still fit in one wave (two waves of parts take longer than
+// one of whole tiles: 1024 x 4096 x 4096 in 64 tiles 37 us split four ways, 22 us whole).
+struct I8PairShape {
+  int m_tiles, n_tiles, bn, tail;
+  long long tiles, cost;  // as plan_i8 counts it
+};
+
+I8PairShape plan_i8_pair(int rows, int n_out, int max_pairs) {
+  I8PairShape p;
+  p.m_tiles = cdiv(rows, I8PairConfig::BN);
+  p.n_tiles = cdiv(n_out, 2 * kBM);
+  p.bn = cdiv(cdiv(rows, p.m_tiles), 32) * 32;
+  p.tiles = (long long)p.m_tiles * p.n_tiles;
+  const long long rest = p.tiles % max_pairs;
+  p.tail = 4;
+  while (p.tail > 1 && (p.bn % (32 * p.tail) != 0 || rest * p.tail > max_pairs)) p.tail /= 2;
+  auto block = [](int bn) { return 32ll + (kBM + bn / 2 > bn ? kBM + bn / 2 : bn); };
+  p.cost = p.tiles / max_pairs * block(p.bn) + (rest > 0 ? block(p.bn / p.tail) : 0);
+  return p;
+}
+
 template <int TN, typename OutT>
 int launch_i8_tn(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, I8Args a, int box, int sm_count,
                  cudaStream_t st) {
@@ -886,19 +908,19 @@ int launch_i8_tn(const void* xq, long long ld_x, const void* wq, long long ld_w,
 }
 
 template <typename OutT>
-int launch_i8_pair(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, I8Args a, int max_pairs,
-                   cudaStream_t st) {
+int launch_i8_pair(const void* xq, long long ld_x, const void* wq, long long ld_w, int K, I8Args a,
+                   const I8PairShape& shape, int max_pairs, cudaStream_t st) {
   int rc = ensure_encode();
   if (rc != DELS_OK) return rc;
   using Cfg = I8PairConfig;
-  a.m_tiles = cdiv(a.rows, Cfg::BN);
-  a.n_tiles = cdiv(a.n_out, 2 * kBM);
+  a.m_tiles = shape.m_tiles;
+  a.n_tiles = shape.n_tiles;
   a.kb = cdiv(K, kI8BK);
-  a.bn = cdiv(cdiv(a.rows, a.m_tiles), 32) * 32;
-  a.tail = a.bn % 128 == 0 ? 4 : (a.bn % 64 == 0 ? 2 : 1);  // split tiles are multiples of 32, too
-  const long long tiles = (long long)a.m_tiles * a.n_tiles;
-  if (tiles > INT32_MAX / 4) return fail(DELS_ERR_UNSUPPORTED, "product of %d rows and %d channels is too large", a.rows, a.n_out);
-  const long long want = tiles < max_pairs ? tiles * a.tail : tiles;
+  a.bn = shape.bn;
+  a.tail = shape.tail;
+  if (shape.tiles > INT32_MAX / 4)
+    return fail(DELS_ERR_UNSUPPORTED, "product of %d rows and %d channels is too large", a.rows, a.n_out);
+  const long long want = shape.tiles < max_pairs ? shape.tiles * a.tail : shape.tiles;
   CUtensorMap mw, mx, mxt;
   if ((rc = make_map_i8(&mw, wq, K, a.n_out, ld_w, kBM)) != DELS_OK) return rc;
   if ((rc = make_map_i8(&mx, xq, K, a.rows, ld_x, a.bn / 2)) != DELS_OK) return rc;
@@ -914,12 +936,11 @@ int launch_i8_out(const void* xq, long long ld_x, const void* wq, long long ld_w
                   int max_pairs, cudaStream_t st) {
   const I8Shape shape = plan_i8(a.rows, a.n_out, sm_count);
   if (a.rows > kBM && max_pairs > 0 && g_use_pairs) {
-    // Pairs where their large tiles fill the device: a pair's block of K costs what a bn-row
-    // tile's does.
-    const int m_tiles = cdiv(a.rows, I8PairConfig::BN), bn = cdiv(cdiv(a.rows, m_tiles), 32) * 32;
-    const long long tiles = (long long)m_tiles * cdiv(a.n_out, 2 * kBM);
-    if (cdiv(tiles, max_pairs) * (32ll + 128 + bn / 2) <= shape.cost + shape.cost / 8)
-      return launch_i8_pair<OutT>(xq, ld_x, wq, ld_w, K, a, max_pairs, st);
+    // Pairs where their tiles are expected to take no longer: K = 4096, pairs against single
+    // CTAs 118 / 137 us for 129 x 151936, 236 / 263 for 512 x 151936, 20 / 23 for 777 x 4096;
+    // but 16 / 10 for 129 x 4096 and 18 / 11 for 777 x 1000, whose tiles leave pairs idle.
+    const I8PairShape pair = plan_i8_pair(a.rows, a.n_out, max_pairs);
+    if (pair.cost <= shape.cost) return launch_i8_pair<OutT>(xq, ld_x, wq, ld_w, K, a, pair, max_pairs, st);
   }
   switch (shape.tn) {
     case 16: return launch_i8_tn<16, OutT>(xq, ld_x, wq, ld_w, K, a, shape.box, sm_count, st);

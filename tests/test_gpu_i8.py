@@ -116,6 +116,19 @@ def test_product_is_exact(cuda_device, out_dtype, rows, K, N):
                   b.float().cpu().numpy())
 
 
+@pytest.mark.parametrize("rows,K,N", [
+    # less than a wave of whole tiles; a second one of whole tiles, of halves, of quarters
+    (200, 130, 12001), (777, 256, 4099), (1024, 129, 5000), (512, 200, 32000), (513, 128, 6501),
+])
+def test_product_in_large_tiles(cuda_device, rows, K, N):
+    from dels_b200 import ops
+
+    dev = cuda_device
+    xq, wq, sx, sw, _, dxq, dwq = make(rows + K + N, rows, K, N, dev)
+    dsx, dsw = torch.from_numpy(sx).to(dev), torch.from_numpy(sw).to(dev)
+    check_product(ops.linear_i8(dxq, dsx, dwq, dsw, out_dtype=torch.float32), xq, wq, sx, sw, None)
+
+
 def test_product_keeps_the_largest_sums(cuda_device):
     """K at its bound with every value at -128: the sum is 2^31 - 2^14, still exact."""
     from dels_b200 import _lib, ops
