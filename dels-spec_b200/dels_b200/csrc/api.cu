@@ -288,8 +288,7 @@ int init_device(int dev) {
     SET(gru_gates_kernel, 0);
     SET(gru_finalize_kernel, 0);
     SET(wait_selftest_kernel, 0);
-    SET_SHARED(beam_reorder_kernel_many(), 0);
-    SET_SHARED(beam_reorder_kernel_few(), 0);
+    SET_SHARED(beam_reorder_kernel, 0);
     for (int i = 0; i < 4; ++i) {
       const bool bf16 = (i & 2) != 0, vec = (i & 1) != 0;
       SET_SHARED(beam_scan_kernel_for(bf16, vec), vec ? kBeamScanSmemMax : 0);
@@ -765,7 +764,8 @@ int launch_beam_select(BeamSelectArgs a, bool bf16, bool shared, bool vec, cudaS
                  launch_pdl(beam_scan_kernel_for(bf16, vec), dim3((unsigned)a.scan_ctas),
                             dim3(32 * scan_pairs(a.scan_rows) * scan_teams(a.scan_rows)),
                             vec ? beam_scan_smem(a.scan_rows, elem, shared) : 0, st, a));
-  // Sixteen warps or nearly: several share a beam's groups where there are few beams.  The bound
+  // Sixteen warps or nearly: several share a beam's groups where there are few beams (1 x 4
+  // beams 11.4 us, 13.3 with a warp for each beam; 64 x 8 beams 48.7 and 51.0).  The bound
   // needs some more maxima than candidates: a lane offers its four quarters' where its
   // largest alone would be too few.
   const int split = a.beams >= kBeamFinishWarps ? 1 : kBeamFinishWarps / a.beams;
@@ -843,7 +843,10 @@ int launch_quantize_rows(const void* x, int dtype, long long ld_x, int rows, int
 // A tile shape of i8_gemm_kernel: rows of a tile and channels that a weight tile loads, and
 // what the whole product then costs: waves of tiles times a block of K's cost, in channels.  A
 // block costs its bytes (box channels, and the rows, which come from L2) and a hand-off worth
-// about 32 channels; wide tiles take at least as long as 128 lanes' MMAs, about TN / 2.
+// about 32 channels (without it 16 x 151936 x 4096 ran in tiles of 8 channels, 351 us instead
+// of 97); wide tiles take at least as long as 128 lanes' MMAs, about TN / 2.  Against every
+// tile of twelve shapes from 3 x 300 to 128 x 151936, the rule's took at most 4 % longer than
+// the best where that is 10 us or more, up to a microsecond longer below.
 struct I8Shape {
   int tn, box;
   long long cost;
@@ -951,7 +954,9 @@ int launch_i8_out(const void* xq, long long ld_x, const void* wq, long long ld_w
   }
 }
 
-// Whether the one-launch form for a few rows takes the product.
+// Whether the one-launch form for a few rows takes the product.  K = 4096, 256 channels: 3.6 us
+// for one row, 4.6 for two, 7.2 for four, against 8.4 of quantising and i8_gemm_kernel; 151936
+// channels: 90, 96 and 196 us (the products bind it, no longer the bytes) against 98.
 bool i8_few_rows(int rows, int K) { return rows <= kI8GemvRows && (long long)rows * ((K + 15) / 16 * 16) <= kI8GemvBytes; }
 
 int launch_i8_gemv(const I8GemvArgs& a, I8Source source, bool out_bf16, int sm_count, cudaStream_t st) {
@@ -1748,7 +1753,7 @@ int dels_beam_reorder(const dels_beam_state* states_in, int n_states, const int3
   const int room = (kBeamReorderSmem / beams - 32) / 128 * 128;
   for (int first = 0; first < n_states; first += kBeamStatesPerLaunch) {
     BeamReorderArgs a = {parents, status, 0, 0, n_seq, beams, select};
-    BeamStates<kBeamStatesPerLaunch> states;
+    BeamStates states;
     for (int i = first; i < n_states && i < first + kBeamStatesPerLaunch; ++i) {
       const dels_beam_state& d = states_in[i];
       if (d.outer == 0 || d.inner_bytes == 0) continue;
@@ -1770,15 +1775,8 @@ int dels_beam_reorder(const dels_beam_state* states_in, int n_states, const int3
     const long long most = (long long)kBeamReorderCtas * ds->sm_count;
     const dim3 grid((unsigned)(a.tiles < most ? a.tiles : most));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (a.n_states <= kBeamFewStates) {
-      BeamStates<kBeamFewStates> few;
-      for (int i = 0; i < a.n_states; ++i) few.st[i] = states.st[i];
-      DELS_CHECK_PDL("beam_reorder_kernel launch",
-                     launch_pdl(beam_reorder_kernel_few(), grid, dim3(kBeamThreads), 0, st, a, few));
-    } else {
-      DELS_CHECK_PDL("beam_reorder_kernel launch",
-                     launch_pdl(beam_reorder_kernel_many(), grid, dim3(kBeamThreads), 0, st, a, states));
-    }
+    DELS_CHECK_PDL("beam_reorder_kernel launch",
+                   launch_pdl(beam_reorder_kernel, grid, dim3(kBeamThreads), 0, st, a, states));
   }
   return DELS_OK;
 }

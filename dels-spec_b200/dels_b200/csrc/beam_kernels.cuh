@@ -10,7 +10,7 @@ constexpr int kBeamMax = 64;         // beams of a sequence, read or selected
 constexpr int kBeamGroup = 512;      // logits of a group, the unit a warp scans at a time
 constexpr int kBeamScanWarps = 4;    // most warps of a scanning CTA
 constexpr int kBeamScanRows = 8;     // most rows a scanning CTA takes together
-constexpr int kBeamScanCtas = 6;     // most scanning CTAs of an SM
+constexpr int kBeamScanCtas = 6;     // most scanning CTAs of an SM: 64 x 8 beams 53 us (5: 60, 7 with a shorter ring: 53, 8: 54)
 constexpr int kBeamFinishWarps = 16; // most warps of a sequence's finishing CTA
 constexpr int kBeamFinishCap = 256;  // quarter groups or candidates it lists before it counts exactly
 constexpr int kBeamListCap = 192;    // counting exactly: quarter groups or logits a warp lists
@@ -71,7 +71,8 @@ struct BeamSelectArgs {
 __host__ __device__ __forceinline__ int scan_pairs(int rows) { return (rows + 1) / 2; }
 __host__ __device__ __forceinline__ int scan_teams(int rows) { return kBeamScanWarps / scan_pairs(rows); }
 
-// The scan's staging rings, one for each team: groups in flight.
+// The scan's staging rings, one for each team: groups in flight, as many as six CTAs of an SM
+// have room for (one of bf16 less made no difference).
 constexpr int beam_scan_depth(int elem) { return elem == 2 ? 3 : 2; }
 // Bytes of a slot: `rows` rows of a group, and the draft logits and prior they share.
 constexpr int beam_slot_bytes(int rows, int elem, bool shared) {
@@ -107,10 +108,9 @@ struct BeamState {
   long long tile0;   // first tile of this state
 };
 
-// States of a launch; a few are passed in a shorter list (copying 2 KB of arguments for each
-// launch costs the host about as much as launching).
+// States of a launch.  Their 2.3 KB of arguments cost nothing that shows: a list of at most four
+// took 3.4 us on the device and 3.7 us of the host's time for two states, as this one does.
 constexpr int kBeamStatesPerLaunch = 32;
-constexpr int kBeamFewStates = 4;
 constexpr int kBeamThreads = 256;
 
 struct BeamReorderArgs {
@@ -120,18 +120,14 @@ struct BeamReorderArgs {
   int n_states;
   int n_seq, beams, select;
 };
-template <int N>
 struct BeamStates {
-  BeamState st[N];
+  BeamState st[kBeamStatesPerLaunch];
 };
 
 // A tile's stage: each beam's piece, up to 15 bytes before it and a word after.
 constexpr int kBeamReorderSmem = 33792;
 constexpr int kBeamReorderCtas = 5;  // an SM holds: 617 MB of a cache in 97 us; a sixth would wait its turn (126 us)
 
-using BeamReorderKernel = void (*)(BeamReorderArgs, BeamStates<kBeamStatesPerLaunch>);
-using BeamReorderFewKernel = void (*)(BeamReorderArgs, BeamStates<kBeamFewStates>);
-BeamReorderKernel beam_reorder_kernel_many();
-BeamReorderFewKernel beam_reorder_kernel_few();
+__global__ void beam_reorder_kernel(const BeamReorderArgs a, const __grid_constant__ BeamStates states);
 
 }  // namespace dels

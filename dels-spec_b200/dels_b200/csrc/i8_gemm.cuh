@@ -12,8 +12,13 @@
 // in a ring; two accumulators in TMEM let a tile's epilogue overlap the next one's MMAs.
 //
 // Warp roles (224 threads): warps 0 and 6 = TMA producers (weights, rows), warp 1 = TMEM
-// allocator + MMA issuer, warps 2..5 = epilogue (one thread per channel).  Above 128 rows CTA pairs share the tiles
-// (i8_pair_kernel).
+// allocator + MMA issuer, warps 2..5 = epilogue (one thread per channel).  Two producers,
+// because one copy takes about 150 cycles to issue: with both operands' on one warp a block of K
+// took 335 cycles, now about 170.
+//
+// Bound by the weights' bytes at few rows: 16 x 151936 x 4096 (625 MB) 97 us, 6.4 TB/s, as
+// a plain copy.  Small products are a chain of latencies (16 x 256 x 4096 8.4 us with the
+// quantisation).  With more than 128 rows CTA pairs may share the tiles (i8_pair_kernel).
 #pragma once
 
 #include "tc_gemm.cuh"
@@ -344,12 +349,16 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 
 // --------------------------------------------------------------------------------
 // The same product on CTA pairs (tcgen05.mma.cta_group::2), for more than 128 rows: a tile is
-// 256 channels x up to 256 rows (a multiple of 32 that the rows fill well), each CTA stages its 128 channels and half of the rows' tile, so a
-// block of K moves 32 KB through each SM's shared memory for the work that takes 48 KB in
-// i8_gemm_kernel.  The barriers are those of tc_scorer_pair_kernel: rank 0 issues the MMAs of
+// 256 channels x up to 256 rows (a multiple of 32 that the rows fill well), each CTA stages its
+// 128 channels and half of the rows' tile, so a block of K moves 32 KB through each SM's shared
+// memory for the work that takes 48 KB in i8_gemm_kernel.  The barriers are those of tc_scorer_pair_kernel: rank 0 issues the MMAs of
 // both CTAs, whose copies complete on rank 0's full barriers.  Two blocks of K form a stage
 // (256 contiguous bytes of every channel).  The last, partial wave's tiles are split along the
 // rows (make_schedule's tail).
+//
+// Bound by the tensor cores and the board's power: 512 x 151936 x 4096 (637 G operations) 217 us
+// at 1.58 GHz with the tensor pipe active 83 % of the cycles, 231-284 us (2.2-2.8 P operations a
+// second) in longer runs, where the clock falls under the power cap.
 // --------------------------------------------------------------------------------
 struct I8PairConfig {
   static constexpr int BN = 256;                 // most rows of a tile
@@ -625,7 +634,7 @@ QuantizeKernel quantize_rows_kernel_for(bool bf16, bool vec);
 constexpr int kI8GemvThreads = 256;
 constexpr int kI8GemvCtas = 3;           // of an SM
 constexpr int kI8GemvRows = 2;           // most rows
-constexpr int kI8GemvBytes = 32768;      // most bytes of quantised rows
+constexpr int kI8GemvBytes = 32768;      // most bytes of quantised rows (an SM's CTAs hold them each)
 enum I8Source { kI8FromInt8 = 0, kI8FromBf16 = 1, kI8FromF32 = 2 };
 struct I8GemvArgs {
   const void* x;        // [rows, K], row stride ld_x elements

@@ -1,10 +1,13 @@
-// Rows to 8-bit integers, and their product with 8-bit weights for a few rows.
-//
+// Rows to 8-bit integers, and their product with 8-bit weights for one or two rows.
 //
 //   a = max_k |x[k]|,  scale = a / 127,  q[k] = rint(x[k] * (127 / a))   (half to even)
 //
 // all in fp32.  A row of zeros has scale 0; a row with NaN or infinity has that scale and
 // q = 0, so what is computed from it is NaN.
+//
+// A block takes a row, reads it twice (the second time from L1 or L2) and writes it once.  512
+// rows of 4096 bf16 take 3.8 us with 16-byte loads and 5.3 us where their alignment rules
+// those out, 16 rows 2.4 and 4.4 us: latency at any size that a draft step has.
 #include "i8_gemm.cuh"
 
 namespace dels {
@@ -30,10 +33,6 @@ __device__ __forceinline__ int to_i8(float x, float inv) {
   const int v = inv == 0.0f ? 0 : __float2int_rn(__fmul_rn(x, inv));
   return max(-127, min(127, v));
 }
-
-}  // namespace
-
-namespace {
 
 // 8 values of a row as int8 (what 16-byte loads give), packed.
 template <typename T>
@@ -100,8 +99,9 @@ QuantizeKernel quantize_rows_kernel_for(bool bf16, bool vec) {
 }
 
 // --------------------------------------------------------------------------------
-// A few rows: y[r, n] = (sum_k xq[r, k] w[n, k]) * sx[r] * sw[n] (+ bias[n]).
-// Bound by the weights' bytes.  A warp reads a channel with 16-byte loads, the next channel's
+// One or two rows: y[r, n] = (sum_k xq[r, k] w[n, k]) * sx[r] * sw[n] (+ bias[n]).
+// Bound by the weights' bytes: 151936 channels of 4096 (622 MB) in 90 us for one row, 6.9 TB/s
+// read, and by latency where they are few: 256 channels in 3.6 us.  A warp reads a channel with 16-byte loads, the next channel's
 // first ones on their way while it adds up, and multiplies by dp4a; the sum is exact.
 // --------------------------------------------------------------------------------
 namespace {
