@@ -924,10 +924,11 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
   __syncthreads();
   if (fill && n_found < n) {
     // The rest are masked tokens, the lowest of the lowest beam.  A beam whose own score is
-    // not finite has other candidates at -inf, which an exact count sorts out.
+    // not finite, or whose lowest logits fall out of fp32 below its maximum, has other candidates
+    // at -inf, which an exact count sorts out.
     const int row = seq * a.beams;
     const bool done = a.finished != nullptr && a.finished[row] != 0;
-    if (warp == 0 && fabsf(f.stat[0].y) < __int_as_float(0x7f800000)) {
+    if (warp == 0 && row_score(-3.402823466e+38f, f.stat[0]) > neg_inf() && f.stat[0].y < -neg_inf()) {
       const Shared<T> sh = shared_terms<T>(a, seq);
       const T* logits = static_cast<const T*>(a.logits) + (long long)row * a.ld;
       int c = n_found;

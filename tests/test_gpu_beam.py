@@ -139,6 +139,22 @@ def test_select_masked_rows(cuda_device, lowest, kept):
     check_select(out, reference_select(np32(logits), cum.numpy(), 8))
 
 
+@pytest.mark.parametrize("V", [1000, 1003])
+def test_select_scores_below_fp32(cuda_device, V):
+    """Logits so far below the row's maximum that their scores fall to -inf: still the larger x
+    first, before masked tokens."""
+    from dels_b200 import ops
+
+    dev = cuda_device
+    x = torch.full((2, V), -INF)
+    x[0, 5], x[0, 7], x[0, 900], x[0, 901] = 3e38, -3e38, -3e38, -2e38
+    x[1, 6] = 1.0
+    out = ops.beam_select(x.to(dev), torch.tensor([[-1.0, -2.0]], device=dev), select=6)
+    assert out.tokens.tolist() == [[5, 6, 901, 7, 900, 0]]
+    assert out.parents.tolist() == [[0, 1, 0, 0, 0, 0]]
+    assert out.scores.tolist() == [[-1.0, -2.0] + [-INF] * 4]
+
+
 def test_select_constant_and_sorted_rows(cuda_device):
     """Equal logits go to the lowest tokens; sorted rows put every candidate in one group."""
     from dels_b200 import ops
