@@ -764,15 +764,26 @@ int launch_beam_select(BeamSelectArgs a, bool bf16, bool shared, bool vec, cudaS
                  launch_pdl(beam_scan_kernel_for(bf16, vec), dim3((unsigned)a.scan_ctas),
                             dim3(32 * scan_pairs(a.scan_rows) * scan_teams(a.scan_rows)),
                             vec ? beam_scan_smem(a.scan_rows, elem, shared) : 0, st, a));
-  // Sixteen warps or nearly: several share a beam's groups where there are few beams (1 x 4
-  // beams 11.4 us, 13.3 with a warp for each beam; 64 x 8 beams 48.7 and 51.0).  The bound
-  // needs some more maxima than candidates: a lane offers its four quarters' where its
-  // largest alone would be too few.
-  const int split = a.beams >= kBeamFinishWarps ? 1 : kBeamFinishWarps / a.beams;
-  const int lanes = a.groups < 32 * split ? a.groups : 32 * split;
+  // The bound needs more maxima than candidates, or it lies low and too many logits reach it.
+  // Where all quarters of all groups offer fewer than twice as many (a small vocabulary), it
+  // comes from the logits themselves: 20 sequences of one beam that take 14 of 1255 logits 17 us
+  // instead of 56.
+  a.finish_direct = 4ll * a.groups * a.beams < 2ll * a.select;
+  // Warps that share a beam: enough for every group, or quarter, to be loaded at once, up to
+  // sixteen for all beams (1 x 4 beams of 151936 logits 11.4 us, 13.3 with a warp for each beam;
+  // 64 x 8 beams 48.7 and 51.0).  More would offer nothing but what they do not have.
+  const int parts = a.finish_direct ? 4 * a.groups : cdiv(a.groups, 32);
+  int split = 1;
+  while (split < parts && 2 * split * a.beams <= kBeamFinishWarps) split *= 2;
   a.finish_split = split;
+  // a lane offers its four quarters' maxima where its largest alone would be too few
+  const int lanes = a.finish_direct || a.groups > 32 * split ? 32 * split : a.groups;
   a.finish_values = a.beams * lanes < 4 * a.select ? 4 : 1;
-  const int warps = split * (a.beams < kBeamFinishWarps ? a.beams : kBeamFinishWarps);
+  // and warps to read the listed quarters together: eight, or one for each candidate
+  const int most = kBeamFinishWarps / split, readers = a.select > 8 ? a.select : 8;
+  int teams = a.beams * split > readers ? a.beams : cdiv(readers, split);
+  if (teams > most) teams = most;
+  const int warps = split * teams;
   DELS_CHECK_PDL("beam_finish_kernel launch",
                  launch_pdl(beam_finish_kernel_for(bf16, vec), dim3((unsigned)a.n_seq), dim3(32 * warps),
                             beam_finish_smem(a.beams, a.select, warps, a.beams * split * 32 * a.finish_values), st, a));

@@ -13,10 +13,9 @@
 //   beam_scan_kernel    one pass over the logits: per slice of a row the running (m, S) of
 //                       an online softmax, and for every 512 logits the maxima of their four
 //                       quarters.
-//   beam_finish_kernel  a CTA per sequence, a warp per beam.  The `select`-th largest of 128
-//                       of those maxima bounds the row's `select` best logits from below, so
-//                       only the quarters that reach it are read again; then the beams' lists
-//                       meet in shared memory.
+//   beam_finish_kernel  a CTA per sequence.  The `select`-th largest score of those maxima, over
+//                       all beams, bounds the sequence's `select` best scores from below, so
+//                       only the quarters that reach it are read again.
 //
 // Both kernels are short loops on purpose: a step of one sequence runs each instruction a
 // few times only, and then fetching code costs more than executing it (unrolled over four
@@ -803,14 +802,26 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
       const float2* row_part = a.ws.part + (long long)row * a.parts;
       float2 p = __ldcg(row_part + min(lane, parts - 1));
       const float4* tops = a.ws.group_top + (long long)row * a.groups;
+      if (a.finish_direct) {
+        const Shared<T> sh = shared_terms<T>(a, seq);
+        const T* logits = static_cast<const T*>(a.logits) + (long long)row * a.ld;
+#pragma unroll 2
+        for (int q = part; q < 4 * a.groups; q += split) {
+          float2 x[2];
+          load_quarter<T, VEC>(a, logits, sh, q, lane, x);
+          top[0] = fmax_nan(top[0], x[0].x), top[1] = fmax_nan(top[1], x[0].y);
+          top[2] = fmax_nan(top[2], x[1].x), top[3] = fmax_nan(top[3], x[1].y);
+        }
+      } else {
 #pragma unroll 1
-      for (int i = part * 32 + lane; i < a.groups; i += kFinishLoads * 32 * split) {
-        float4 t[kFinishLoads];
-        load_tops(tops, i, 32 * split, a.groups, t);
+        for (int i = part * 32 + lane; i < a.groups; i += kFinishLoads * 32 * split) {
+          float4 t[kFinishLoads];
+          load_tops(tops, i, 32 * split, a.groups, t);
 #pragma unroll
-        for (int u = 0; u < kFinishLoads; ++u) {
-          top[0] = fmax_nan(top[0], t[u].x), top[1] = fmax_nan(top[1], t[u].y);
-          top[2] = fmax_nan(top[2], t[u].z), top[3] = fmax_nan(top[3], t[u].w);
+          for (int u = 0; u < kFinishLoads; ++u) {
+            top[0] = fmax_nan(top[0], t[u].x), top[1] = fmax_nan(top[1], t[u].y);
+            top[2] = fmax_nan(top[2], t[u].z), top[3] = fmax_nan(top[3], t[u].w);
+          }
         }
       }
       if (lane >= parts) p = make_float2(neg_inf(), 0.0f);
@@ -883,7 +894,7 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
       }
       // few lanes hold a maximum that reaches the bound
       const uint32_t* value = f.value + ((k * split + part) * 32 + lane) * per_lane;
-      if (value[0] < key && (per_lane == 1 || max(max(value[1], value[2]), value[3]) < key)) continue;
+      if (!a.finish_direct && value[0] < key && (per_lane == 1 || max(max(value[1], value[2]), value[3]) < key)) continue;
       const float4* tops = a.ws.group_top + (long long)row * a.groups;
 #pragma unroll 1
       for (int i = part * 32 + lane; i < a.groups; i += kFinishLoads * 32 * split) {

@@ -57,8 +57,9 @@ struct BeamSelectArgs {
   int scan_rows;             // rows of a block, scanned together
   int scan_ctas;
   ScanShare share;
-  int finish_split;          // warps of the finishing CTA that share a beam
-  int finish_values;         // group maxima a lane of them offers for the bound
+  int finish_split;          // warps of the finishing CTA that share a beam; it has a multiple of them
+  int finish_direct;         // the bound comes from the logits themselves, not from group maxima
+  int finish_values;         // maxima a lane of them offers for it
   int slot_bytes;            // of its staging ring
   int* status;               // device error word
   int* parents;              // [n_seq, select]

@@ -355,7 +355,8 @@ DELS_API int dels_correction_mid_tc_bf16(const void* h, int64_t ld_h, const void
  *   dels_linear_i8          out[i, n] = (sum_k xq[i, k] wq[n, k]) * x_scale[i] * w_scale[n]
  *                           (+ bias[n]); the sum is exact, in 32-bit integers.
  *   dels_linear_w8a8        both: quantises x into the workspace, then the product, which
- *                           starts to load the weights while x is being quantised.
+ *                           starts to load the weights while x is being quantised (one or
+ *                           two rows: one kernel that does both).
  * x [rows, K] bf16 or fp32 with any row stride; q / xq / wq int8 with 16-byte aligned
  * rows (ld % 16 == 0); out and bias bf16 or fp32 (out_dtype), any row stride.
  * K <= DELS_I8_MAX_K.  ws: DELS_WS_HEADER_BYTES for dels_linear_i8,

@@ -139,6 +139,27 @@ def test_select_masked_rows(cuda_device, lowest, kept):
     check_select(out, reference_select(np32(logits), cum.numpy(), 8))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n_seq,beams,select,V", [
+    (20, 1, 14, 1255), (31, 1, 27, 3920), (9, 2, 29, 1064), (2, 3, 64, 1100), (200, 2, 2, 1689), (3, 5, 40, 530),
+    (2, 1, 64, 16384), (2, 1, 64, 16392),
+])
+def test_select_many_of_a_small_vocabulary(cuda_device, dtype, n_seq, beams, select, V):
+    """More candidates than there are groups of logits, half of the vocabulary masked, some beams
+    finished."""
+    from dels_b200 import ops
+
+    dev = cuda_device
+    rng, logits, base, prior, cum = make(V + select, n_seq, beams, V, dtype, True, dev)
+    logits[:, torch.from_numpy(rng.permutation(V)[: V // 2])] = -INF
+    finished = torch.from_numpy(rng.random((n_seq, beams)) < 0.3)
+    beta = torch.tensor([0.2], device=dev)
+    out = ops.beam_select(logits.to(dev), cum.to(dev), select=select, base=base.to(dev), prior=prior.to(dev),
+                          beta=beta, finished=finished.to(dev), pad_token=2)
+    check_select(out, reference_select(np32(logits), cum.numpy(), select, np32(base), prior.numpy(), 0.2,
+                                       finished.numpy(), 2))
+
+
 @pytest.mark.parametrize("V", [1000, 1003])
 def test_select_scores_below_fp32(cuda_device, V):
     """Logits so far below the row's maximum that their scores fall to -inf: still the larger x
