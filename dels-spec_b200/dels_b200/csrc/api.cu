@@ -295,8 +295,8 @@ int init_device(int dev) {
       SET_SHARED(beam_finish_kernel_for(bf16, vec), kBeamFinishSmemMax);
       SET(quantize_rows_kernel_for(bf16, vec), 0);
     }
-    for (int i = 0; i < 12; ++i)
-      SET(i8_gemv_kernel_for((I8Source)(i % 3), (i / 3 & 1) != 0, 1 << i / 6), kI8GemvBytes);
+    for (int i = 0; i < 36; ++i)
+      SET(i8_gemv_kernel_for((I8Source)(i % 3), (i / 3 & 1) != 0, 1 + i / 6 % 2, 1 << i / 12), kI8GemvBytes);
     SET((i8_gemm_kernel<16, __nv_bfloat16>), I8Config<16>::kMaxBytes);
     SET((i8_gemm_kernel<32, __nv_bfloat16>), I8Config<32>::kMaxBytes);
     SET((i8_gemm_kernel<64, __nv_bfloat16>), I8Config<64>::kMaxBytes);
@@ -968,12 +968,20 @@ int launch_i8_out(const void* xq, long long ld_x, const void* wq, long long ld_w
 // Whether the one-launch form for a few rows takes the product.  K = 4096, 256 channels: 3.6 us
 // for one row, 4.6 for two, 7.2 for four, against 8.4 of quantising and i8_gemm_kernel; 151936
 // channels: 90, 96 and 196 us (the products bind it, no longer the bytes) against 98.
-bool i8_few_rows(int rows, int K) { return rows <= kI8GemvRows && (long long)rows * ((K + 15) / 16 * 16) <= kI8GemvBytes; }
+bool i8_few_rows(int rows, int K, int N) {
+  return rows <= kI8GemvRows && (long long)rows * ((K + 15) / 16 * 16) <= kI8GemvBytes && N <= (1 << 30);
+}
 
 int launch_i8_gemv(const I8GemvArgs& a, I8Source source, bool out_bf16, int sm_count, cudaStream_t st) {
-  const int most = kI8GemvCtas * sm_count, want = cdiv(a.n_out, kI8GemvThreads / 32);
+  // A warp takes as many channels together as its loads in flight cover, while every warp still
+  // has some: 119104 channels of K = 768 19 us, 47 one at a time.
+  const int most = kI8GemvCtas * sm_count, warps = kI8GemvThreads / 32;
+  int channels = 1;
+  while (channels < 4 && 2 * channels * cdiv(a.K, 512) <= kI8GemvLoads && a.n_out >= 2 * channels * most * warps)
+    channels *= 2;
+  const int want = cdiv(a.n_out, warps * channels);
   DELS_CHECK_PDL("i8_gemv_kernel launch",
-                 launch_pdl(i8_gemv_kernel_for(source, out_bf16, a.rows), dim3(want < most ? want : most),
+                 launch_pdl(i8_gemv_kernel_for(source, out_bf16, a.rows, channels), dim3(want < most ? want : most),
                             dim3(kI8GemvThreads), (size_t)a.rows * ((a.K + 15) / 16 * 16), st, a));
   return DELS_OK;
 }
@@ -1822,7 +1830,7 @@ int dels_linear_i8(const int8_t* xq, int64_t ld_xq, const float* x_scale, const 
   DeviceState* ds = nullptr;
   if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
   if (rows == 0) return DELS_OK;
-  if (i8_few_rows(rows, K))
+  if (i8_few_rows(rows, K, N))
     return launch_i8_gemv({xq, ld_xq, 1, x_scale, wq, ld_wq, w_scale, bias, out, ld_out, rows, K, N}, kI8FromInt8,
                           out_dtype == DELS_DTYPE_BF16, ds->sm_count, reinterpret_cast<cudaStream_t>(stream));
   // the kernel before this one may be the one that quantised the weights
@@ -1847,7 +1855,7 @@ int dels_linear_w8a8(const void* x, int x_dtype, int64_t ld_x, const int8_t* wq,
   if ((rc = ws_header(ws, ws_bytes, dels_linear_w8a8_workspace_bytes(rows, K), &hdr)) != DELS_OK) return rc;
   DeviceState* ds = nullptr;
   if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
-  if (rows > 0 && i8_few_rows(rows, K)) {
+  if (rows > 0 && i8_few_rows(rows, K, N)) {
     if ((rc = check_quantize(x, x_dtype, ld_x, rows, K)) != DELS_OK) return rc;
     const bool vec = aligned16(x) && (ld_x * (x_dtype == DELS_DTYPE_BF16 ? 2 : 4)) % 16 == 0;
     return launch_i8_gemv({x, ld_x, vec, nullptr, wq, ld_wq, w_scale, bias, out, ld_out, rows, K, N},

@@ -629,10 +629,11 @@ using QuantizeKernel = void (*)(const void* x, long long ld_x, int rows, int K, 
 QuantizeKernel quantize_rows_kernel_for(bool bf16, bool vec);
 
 // A few rows against all channels in one launch: each CTA quantises the rows for itself (or
-// copies quantised ones) into shared memory, then a warp takes a channel at a time with
-// dp4a (i8_kernels.cu).
+// copies quantised ones) into shared memory, then a warp takes one, two or four channels at a
+// time with dp4a (i8_kernels.cu).
 constexpr int kI8GemvThreads = 256;
 constexpr int kI8GemvCtas = 3;           // of an SM
+constexpr int kI8GemvLoads = 8;          // 16-byte loads of a lane in flight
 constexpr int kI8GemvRows = 2;           // most rows
 constexpr int kI8GemvBytes = 32768;      // most bytes of quantised rows (an SM's CTAs hold them each)
 enum I8Source { kI8FromInt8 = 0, kI8FromBf16 = 1, kI8FromF32 = 2 };
@@ -650,6 +651,6 @@ struct I8GemvArgs {
   int rows, K, n_out;
 };
 using I8GemvKernel = void (*)(I8GemvArgs);
-I8GemvKernel i8_gemv_kernel_for(I8Source source, bool out_bf16, int rows);
+I8GemvKernel i8_gemv_kernel_for(I8Source source, bool out_bf16, int rows, int channels);
 
 }  // namespace dels

@@ -114,22 +114,27 @@ __device__ __forceinline__ uint4 load_weights(const int8_t* p) {
   return w;
 }
 
-// dynamic shared memory: [ROWS][padded K] quantised rows, zero past K
-template <typename T, typename OutT, int ROWS>
+// ROWS: most rows; G: channels that a warp takes at a time, with kI8GemvLoads / G loads of a lane
+// for each.  Dynamic shared memory: [ROWS][padded K] quantised rows, zero past K.
+template <typename T, typename OutT, int ROWS, int G>
 __global__ void __launch_bounds__(kI8GemvThreads, kI8GemvCtas) i8_gemv_kernel(I8GemvArgs a) {
   constexpr int kWarps = kI8GemvThreads / 32;
-  constexpr int U = 8;  // 16-byte loads of a lane in flight
+  constexpr int U = kI8GemvLoads, S = U / G;
   extern __shared__ __align__(16) int8_t rows_q[];
   __shared__ float warp_top[kWarps], scale[ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int padded = (a.K + 15) / 16 * 16, chunks = padded / 16, whole = a.K / 16;
-  int n = blockIdx.x * kWarps + warp;
+  int n = (blockIdx.x * kWarps + warp) * G;
   uint4 w[U];
-  auto fetch = [&](int channel, int c0) {
+  // Chunks of 16 bytes of the channels from n0 on.  The last, partial one of a channel reaches
+  // into the row's padding, whose products with the rows' zeros vanish; the last channel, with
+  // no padding to rely on, adds its last bytes one by one.
+  auto fetch = [&](int n0, int c0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int c = c0 + u * 32 + lane;
-      w[u] = channel < a.n_out && c < whole ? load_weights(a.w + (long long)channel * a.ld_w + 16 * c) : make_uint4(0, 0, 0, 0);
+      const int channel = n0 + u / S, c = c0 + u % S * 32 + lane;
+      const int end = channel + 1 < a.n_out ? chunks : (channel < a.n_out ? whole : 0);
+      w[u] = c < end ? load_weights(a.w + (long long)channel * a.ld_w + 16 * c) : make_uint4(0, 0, 0, 0);
     }
   };
   pdl_wait();  // (the kernel before this one may be the one that quantised the weights)
@@ -152,54 +157,57 @@ __global__ void __launch_bounds__(kI8GemvThreads, kI8GemvCtas) i8_gemv_kernel(I8
     for (int k = a.K + threadIdx.x; k < padded; k += kI8GemvThreads) dst[k] = 0;
   }
   __syncthreads();
-  const int step = gridDim.x * kWarps;
+  const int step = gridDim.x * kWarps * G;
 #pragma unroll 1
   for (; n < a.n_out; n += step) {
-    int acc[ROWS] = {};
-    for (int c0 = 0; c0 < chunks; c0 += 32 * U) {
+    int acc[G][ROWS] = {};
+    for (int c0 = 0; c0 < chunks; c0 += 32 * S) {
       uint4 v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) v[u] = w[u];
-      // a channel's last, partial 16 bytes come byte by byte
-      const int last = whole - c0;
-      if (whole < chunks && last >= 0 && last < 32 * U && (last & 31) == lane) {
-        const int8_t* p = a.w + (long long)n * a.ld_w + 16 * whole;
-        uint32_t b[4] = {0, 0, 0, 0};
+      const bool more = c0 + 32 * S < chunks;
+      fetch(more ? n : n + step, more ? c0 + 32 * S : 0);
 #pragma unroll
-        for (int j = 0; j < 15; ++j)
-          if (j < a.K - 16 * whole) b[j >> 2] |= (uint32_t)(uint8_t)p[j] << (8 * (j & 3));
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (u == last >> 5) v[u] = make_uint4(b[0], b[1], b[2], b[3]);
-      }
-      const bool more = c0 + 32 * U < chunks;
-      fetch(more ? n : n + step, more ? c0 + 32 * U : 0);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = c0 + u * 32 + lane;
+      for (int s = 0; s < S; ++s) {
+        const int c = c0 + s * 32 + lane;
         if (c < chunks) {
 #pragma unroll
           for (int r = 0; r < ROWS; ++r) {
             if (r >= a.rows) break;
             const uint4 x = reinterpret_cast<const uint4*>(rows_q + r * padded)[c];
-            acc[r] = __dp4a((int)v[u].x, (int)x.x, acc[r]);
-            acc[r] = __dp4a((int)v[u].y, (int)x.y, acc[r]);
-            acc[r] = __dp4a((int)v[u].z, (int)x.z, acc[r]);
-            acc[r] = __dp4a((int)v[u].w, (int)x.w, acc[r]);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const uint4 y = v[g * S + s];
+              acc[g][r] = __dp4a((int)y.x, (int)x.x, acc[g][r]);
+              acc[g][r] = __dp4a((int)y.y, (int)x.y, acc[g][r]);
+              acc[g][r] = __dp4a((int)y.z, (int)x.z, acc[g][r]);
+              acc[g][r] = __dp4a((int)y.w, (int)x.w, acc[g][r]);
+            }
           }
         }
       }
     }
-    int mine = 0;  // lane r: the sum of row r
+    if (n + G >= a.n_out && 16 * whole + lane < a.K) {
+      const int k = 16 * whole + lane, byte = a.w[(long long)(a.n_out - 1) * a.ld_w + k];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-      const int total = __reduce_add_sync(0xffffffffu, acc[r]);
-      mine = lane == r ? total : mine;
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          if (r < a.rows && n + g == a.n_out - 1) acc[g][r] += byte * rows_q[r * padded + k];
     }
-    if (lane < a.rows) {
-      float y = __int2float_rn(mine) * scale[lane] * a.sw[n];
-      if (a.bias != nullptr) y += to_f32(static_cast<const OutT*>(a.bias)[n]);
-      OutT* out = static_cast<OutT*>(a.out) + (long long)lane * a.ld_out + n;
+    int mine = 0;  // lane G r + g: the sum of row r and channel g
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const int total = __reduce_add_sync(0xffffffffu, acc[g][r]);
+        mine = lane == G * r + g ? total : mine;
+      }
+    const int r = lane / G, channel = n + lane % G;
+    if (r < a.rows && channel < a.n_out) {
+      float y = __int2float_rn(mine) * scale[r] * a.sw[channel];
+      if (a.bias != nullptr) y += to_f32(static_cast<const OutT*>(a.bias)[channel]);
+      OutT* out = static_cast<OutT*>(a.out) + (long long)r * a.ld_out + channel;
       if constexpr (sizeof(OutT) == 2)
         *out = __float2bfloat16_rn(y);
       else
@@ -208,21 +216,27 @@ __global__ void __launch_bounds__(kI8GemvThreads, kI8GemvCtas) i8_gemv_kernel(I8
   }
 }
 
+template <typename T, typename OutT, int ROWS>
+I8GemvKernel i8_gemv_channels(int channels) {
+  if (channels == 4) return i8_gemv_kernel<T, OutT, ROWS, 4>;
+  return channels == 2 ? i8_gemv_kernel<T, OutT, ROWS, 2> : i8_gemv_kernel<T, OutT, ROWS, 1>;
+}
+
 template <typename T, typename OutT>
-I8GemvKernel i8_gemv_rows(int rows) {
-  return rows <= 1 ? i8_gemv_kernel<T, OutT, 1> : i8_gemv_kernel<T, OutT, 2>;
+I8GemvKernel i8_gemv_rows(int rows, int channels) {
+  return rows <= 1 ? i8_gemv_channels<T, OutT, 1>(channels) : i8_gemv_channels<T, OutT, 2>(channels);
 }
 
 }  // namespace
 
-I8GemvKernel i8_gemv_kernel_for(I8Source source, bool out_bf16, int rows) {
+I8GemvKernel i8_gemv_kernel_for(I8Source source, bool out_bf16, int rows, int channels) {
   switch (source) {
     case kI8FromInt8:
-      return out_bf16 ? i8_gemv_rows<int8_t, __nv_bfloat16>(rows) : i8_gemv_rows<int8_t, float>(rows);
+      return out_bf16 ? i8_gemv_rows<int8_t, __nv_bfloat16>(rows, channels) : i8_gemv_rows<int8_t, float>(rows, channels);
     case kI8FromBf16:
-      return out_bf16 ? i8_gemv_rows<__nv_bfloat16, __nv_bfloat16>(rows) : i8_gemv_rows<__nv_bfloat16, float>(rows);
+      return out_bf16 ? i8_gemv_rows<__nv_bfloat16, __nv_bfloat16>(rows, channels) : i8_gemv_rows<__nv_bfloat16, float>(rows, channels);
     default:
-      return out_bf16 ? i8_gemv_rows<float, __nv_bfloat16>(rows) : i8_gemv_rows<float, float>(rows);
+      return out_bf16 ? i8_gemv_rows<float, __nv_bfloat16>(rows, channels) : i8_gemv_rows<float, float>(rows, channels);
   }
 }
 

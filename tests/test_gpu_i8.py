@@ -116,6 +116,30 @@ def test_product_is_exact(cuda_device, out_dtype, rows, K, N):
                   b.float().cpu().numpy())
 
 
+@pytest.mark.parametrize("source", [torch.int8, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,K,N", [
+    (1, 768, 30001), (2, 1000, 20003), (1, 1500, 9001), (2, 2047, 7777), (1, 130, 14211), (2, 15, 15000), (1, 1024, 7103),
+])
+def test_product_of_few_rows_and_many_channels(cuda_device, source, rows, K, N):
+    """One or two rows take several channels at a time; the last channel's row of the weights
+    ends with its last value."""
+    from dels_b200 import ops
+
+    dev = cuda_device
+    xq, wq, sx, sw, _, dxq, dwq = make(rows + K + N, rows, K, N, dev)
+    ld = -(-K // 16) * 16
+    tight = torch.empty((N - 1) * ld + K, dtype=torch.int8, device=dev)
+    w = tight.as_strided((N, K), (ld, 1))
+    w.copy_(dwq)
+    dsx, dsw = torch.from_numpy(sx).to(dev), torch.from_numpy(sw).to(dev)
+    if source == torch.int8:
+        check_product(ops.linear_i8(dxq, dsx, w, dsw, out_dtype=torch.float32), xq, wq, sx, sw, None)
+        return
+    x = (dxq.float() * dsx[:, None]).to(source)
+    q, scale = ops.quantize_rows_i8(x)
+    check_product(ops.linear_w8a8(x, w, dsw, out_dtype=torch.float32), q.cpu().numpy(), wq, scale.cpu().numpy(), sw, None)
+
+
 @pytest.mark.parametrize("rows,K,N", [
     # less than a wave of whole tiles; a second one of whole tiles, of halves, of quarters
     (200, 130, 12001), (777, 256, 4099), (1024, 129, 5000), (512, 200, 32000), (513, 128, 6501),
