@@ -297,18 +297,18 @@ int init_device(int dev) {
     }
     for (int i = 0; i < 36; ++i)
       SET(i8_gemv_kernel_for((I8Source)(i % 3), (i / 3 & 1) != 0, 1 + i / 6 % 2, 1 << i / 12), kI8GemvBytes);
-    SET((i8_gemm_kernel<16, __nv_bfloat16>), I8Config<16>::kMaxBytes);
-    SET((i8_gemm_kernel<32, __nv_bfloat16>), I8Config<32>::kMaxBytes);
-    SET((i8_gemm_kernel<64, __nv_bfloat16>), I8Config<64>::kMaxBytes);
-    SET((i8_gemm_kernel<128, __nv_bfloat16>), I8Config<128>::kMaxBytes);
-    SET((i8_gemm_kernel<256, __nv_bfloat16>), I8Config<256>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<16, __nv_bfloat16>), I8Config<16>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<32, __nv_bfloat16>), I8Config<32>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<64, __nv_bfloat16>), I8Config<64>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<128, __nv_bfloat16>), I8Config<128>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<256, __nv_bfloat16>), I8Config<256>::kMaxBytes);
     SET(i8_pair_kernel<__nv_bfloat16>, I8PairConfig::kSmemBytes);
     SET(i8_pair_kernel<float>, I8PairConfig::kSmemBytes);
-    SET((i8_gemm_kernel<16, float>), I8Config<16>::kMaxBytes);
-    SET((i8_gemm_kernel<32, float>), I8Config<32>::kMaxBytes);
-    SET((i8_gemm_kernel<64, float>), I8Config<64>::kMaxBytes);
-    SET((i8_gemm_kernel<128, float>), I8Config<128>::kMaxBytes);
-    SET((i8_gemm_kernel<256, float>), I8Config<256>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<16, float>), I8Config<16>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<32, float>), I8Config<32>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<64, float>), I8Config<64>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<128, float>), I8Config<128>::kMaxBytes);
+    SET_SHARED((i8_gemm_kernel<256, float>), I8Config<256>::kMaxBytes);
 #undef SET
 #undef SET_SHARED
   }
@@ -914,10 +914,15 @@ int launch_i8_tn(const void* xq, long long ld_x, const void* wq, long long ld_w,
   if ((rc = make_map_i8(&mx, xq, K, a.rows, ld_x, TN)) != DELS_OK) return rc;
   const long long units = (long long)a.n_tiles * a.m_tiles;
   if (units > INT32_MAX) return fail(DELS_ERR_UNSUPPORTED, "product of %d rows and %d channels is too large", a.rows, a.n_out);
+  // A small K leaves room for several CTAs of an SM, whose epilogues then overlap: 101 x 146496 x
+  // 64 24 us, 37 with one.
+  const int smem = I8Config<TN>::kFixedBytes + a.stages * I8Config<TN>::slot_bytes(box);
+  const int by_smem = (220 << 10) / (smem + 1024), by_tmem = 512 / I8Config<TN>::kTmemCols;
+  const int ctas = by_smem < by_tmem ? by_smem : by_tmem;
+  const long long most = (long long)sm_count * (ctas < 1 ? 1 : (ctas < kI8MostCtas ? ctas : kI8MostCtas));
   DELS_CHECK_PDL("i8_gemm_kernel launch",
-                 launch_pdl(i8_gemm_kernel<TN, OutT>, dim3((unsigned)(units < sm_count ? units : sm_count)),
-                            dim3(kI8Threads), I8Config<TN>::kFixedBytes + a.stages * I8Config<TN>::slot_bytes(box), st,
-                            mw, mx, a));
+                 launch_pdl(i8_gemm_kernel<TN, OutT>, dim3((unsigned)(units < most ? units : most)), dim3(kI8Threads),
+                            smem, st, mw, mx, a));
   return DELS_OK;
 }
 

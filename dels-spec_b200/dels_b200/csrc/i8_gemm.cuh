@@ -45,6 +45,7 @@ struct I8Args {
 };
 
 constexpr int kI8MaxStages = 32;
+constexpr int kI8MostCtas = 4;  // of an SM
 
 // Shared memory: the barriers and the row scales, then the ring: args.stages weight slots of
 // args.box lines, 16 KB for the lanes that the last of them leaves unloaded, the rows' slots.
@@ -106,7 +107,8 @@ __host__ __device__ constexpr uint32_t make_idesc_s8_s32(int M, int N) {
          | ((uint32_t)(M >> 4) << 24);    // M / 16
 }
 
-// One channel's results for the COLS rows row0.. of a tile (`valid` of them exist).
+// One channel's results for the COLS rows row0.. of a tile; `valid` of them exist, the others
+// are computed all the same and not stored, so that no branch keeps the rows' chains apart.
 template <int COLS, typename OutT>
 __device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float* scale, float sw, float bias, int valid,
                                          bool channel_ok, OutT* out, long long ld, bool store2, int lane) {
@@ -117,7 +119,6 @@ __device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float*
       const bool odd = lane & 1;
 #pragma unroll
       for (int j = 0; j < COLS; j += 2) {
-        if (j >= valid) break;
         const float y0 = __int2float_rn((int)v[j]) * scale[j] * sw + bias;
         const float y1 = __int2float_rn((int)v[j + 1]) * scale[j + 1] * sw + bias;
         const float other = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 1);
@@ -130,9 +131,8 @@ __device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float*
   }
 #pragma unroll
   for (int j = 0; j < COLS; ++j) {
-    if (j >= valid) break;
     const float y = __int2float_rn((int)v[j]) * scale[j] * sw + bias;
-    if (channel_ok) {
+    if (channel_ok && j < valid) {
       if constexpr (sizeof(OutT) == 2)
         out[j * ld] = __float2bfloat16_rn(y);
       else
