@@ -642,7 +642,8 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
         const int j = __ffs((int)reach) - 1;
         const float y = j & 2 ? (j & 1 ? x[1].y : x[1].x) : (j & 1 ? x[0].y : x[0].x);
         const int slot = atomicAdd(w.count, 1);
-        if (slot < kBeamListCap) w.list[slot] = entry_key(ordered_u32(y), (q >> 2) * kBeamGroup + quarter_offset<VEC>(q & 3, lane, j));
+        const int token = (q >> 2) * kBeamGroup + quarter_offset<VEC>(q & 3, lane, j);
+        if (slot < kBeamListCap) w.list[slot] = entry_key(ordered_u32(y), token);
       }
     });
     __syncwarp();
@@ -758,13 +759,14 @@ __device__ __noinline__ void finish_exact(const BeamSelectArgs& a, const FinishS
 }  // namespace
 
 // A CTA per sequence; `finish_split` warps share a beam's groups.  The scores of group maxima,
-// over all beams, bound the sequence's `select` best scores from below; few quarters reach the
-// bound (about `select` of all beams together), and only they are read again, a warp each.
+// over all beams (of small vocabularies the logits'), bound the sequence's `select` best scores
+// from below; few quarters reach the bound (about `select` of all beams together), and only
+// they are read again, a warp each.
 // Where the bound says little (masked rows, many equal scores, more candidates than the list
 // holds) the CTA counts exactly, beam by beam.
 //
-// About 6 us for 64 x 8 or 1 x 4 beams of 151936 logits: a chain of dependent loads (maxima,
-// bound, quarters), which the number of warps shortens.
+// About 7 us for 64 x 8 or 1 x 4 beams of 151936 logits: a chain of dependent loads (maxima,
+// bound, quarters), which more warps shorten.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(BeamSelectArgs a) {
   extern __shared__ __align__(16) char smem[];
@@ -894,7 +896,9 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(Beam
       }
       // few lanes hold a maximum that reaches the bound
       const uint32_t* value = f.value + ((k * split + part) * 32 + lane) * per_lane;
-      if (!a.finish_direct && value[0] < key && (per_lane == 1 || max(max(value[1], value[2]), value[3]) < key)) continue;
+      if (!a.finish_direct && value[0] < key &&
+          (per_lane == 1 || max(max(value[1], value[2]), value[3]) < key))
+        continue;
       const float4* tops = a.ws.group_top + (long long)row * a.groups;
 #pragma unroll 1
       for (int i = part * 32 + lane; i < a.groups; i += kFinishLoads * 32 * split) {

@@ -10,7 +10,8 @@ constexpr int kBeamMax = 64;         // beams of a sequence, read or selected
 constexpr int kBeamGroup = 512;      // logits of a group, the unit a warp scans at a time
 constexpr int kBeamScanWarps = 4;    // most warps of a scanning CTA
 constexpr int kBeamScanRows = 8;     // most rows a scanning CTA takes together
-constexpr int kBeamScanCtas = 6;     // most scanning CTAs of an SM: 64 x 8 beams 53 us (5: 60, 7 with a shorter ring: 53, 8: 54)
+// Most scanning CTAs of an SM: 64 x 8 beams 53 us (5: 60, 7 with a shorter ring: 53, 8: 54).
+constexpr int kBeamScanCtas = 6;
 constexpr int kBeamFinishWarps = 16; // most warps of a sequence's finishing CTA
 constexpr int kBeamFinishCap = 256;  // quarter groups or candidates it lists before it counts exactly
 constexpr int kBeamListCap = 192;    // counting exactly: quarter groups or logits a warp lists

@@ -351,10 +351,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 // The same product on CTA pairs (tcgen05.mma.cta_group::2), for more than 128 rows: a tile is
 // 256 channels x up to 256 rows (a multiple of 32 that the rows fill well), each CTA stages its
 // 128 channels and half of the rows' tile, so a block of K moves 32 KB through each SM's shared
-// memory for the work that takes 48 KB in i8_gemm_kernel.  The barriers are those of tc_scorer_pair_kernel: rank 0 issues the MMAs of
-// both CTAs, whose copies complete on rank 0's full barriers.  Two blocks of K form a stage
-// (256 contiguous bytes of every channel).  The last, partial wave's tiles are split along the
-// rows (make_schedule's tail).
+// memory for the work that takes 48 KB in i8_gemm_kernel.  The barriers are those of
+// tc_scorer_pair_kernel: rank 0 issues the MMAs of both CTAs, whose copies complete on rank 0's
+// full barriers.  Two blocks of K form a stage (256 contiguous bytes of every channel).  The
+// last, partial wave's tiles are split along the rows (make_schedule's tail).
 //
 // Bound by the tensor cores and the board's power: 512 x 151936 x 4096 (637 G operations) 217 us
 // at 1.58 GHz with the tensor pipe active 83 % of the cycles, 231-284 us (2.2-2.8 P operations a
