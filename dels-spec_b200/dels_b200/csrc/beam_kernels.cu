@@ -607,62 +607,76 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
       top[2] = max(top[2], ordered_u32(x[1].x)), top[3] = max(top[3], ordered_u32(x[1].y));
     });
   }
-  uint32_t bound = warp_bound(top, a.select);
-  // Too little above -inf: take all that is, and the lowest masked tokens for the rest.
-  const bool fill = bound <= none;
+  uint32_t bound = warp_bound(top, a.select), rest = none;
+  // With too little above -inf: all that is, and the lowest masked tokens.  Where more logits than
+  // the list holds reach the bound, many of them mostly equal it (a mask of the type's lowest value,
+  // constant rows): those above it, and the lowest tokens of the rest, 64 x 1 beams that take 16 with
+  // one token allowed 59 us instead of 618.
+  bool fill = bound <= none;
   if (fill) bound = none + 1;
-  const float floor = ordered_u32_to_float(bound);
-  int n_list = 4 * a.groups;
-  if (!few) {
-    if (lane == 0) *w.count = 0;
-    __syncwarp();
 #pragma unroll 1
-    for (int i = lane; i < a.groups; i += 32) {
-      const float4 t = __ldcg(tops + i);
-      // NaN counts as above every bound
-      uint32_t reach = (t.x < floor ? 0u : 1u) | (t.y < floor ? 0u : 2u) | (t.z < floor ? 0u : 4u) | (t.w < floor ? 0u : 8u);
+  while (true) {
+    const float floor = ordered_u32_to_float(bound);
+    int n_list = 4 * a.groups;
+    if (!few) {
+      if (lane == 0) *w.count = 0;
+      __syncwarp();
 #pragma unroll 1
-      for (; reach != 0; reach &= reach - 1) {
-        const int slot = atomicAdd(w.count, 1);
-        if (slot < kBeamListCap) w.quarters[slot] = 4 * i + __ffs((int)reach) - 1;
-      }
-    }
-    __syncwarp();
-    n_list = *w.count;
-    __syncwarp();
-  }
-  if (lane == 0) *w.count = 0;
-  __syncwarp();
-  if (n_list <= kBeamListCap) {
-    each_quarter<T, VEC>(a, logits, sh, w.quarters, n_list, [&](const float2(&x)[2], int q) {
-      uint32_t reach = (x[0].x < floor ? 0u : 1u) | (x[0].y < floor ? 0u : 2u) | (x[1].x < floor ? 0u : 4u) |
-                       (x[1].y < floor ? 0u : 8u);
+      for (int i = lane; i < a.groups; i += 32) {
+        const float4 t = __ldcg(tops + i);
+        // NaN counts as above every bound
+        uint32_t reach =
+            (t.x < floor ? 0u : 1u) | (t.y < floor ? 0u : 2u) | (t.z < floor ? 0u : 4u) | (t.w < floor ? 0u : 8u);
 #pragma unroll 1
-      for (; reach != 0; reach &= reach - 1) {
-        const int j = __ffs((int)reach) - 1;
-        const float y = j & 2 ? (j & 1 ? x[1].y : x[1].x) : (j & 1 ? x[0].y : x[0].x);
-        const int slot = atomicAdd(w.count, 1);
-        const int token = (q >> 2) * kBeamGroup + quarter_offset<VEC>(q & 3, lane, j);
-        if (slot < kBeamListCap) w.list[slot] = entry_key(ordered_u32(y), token);
-      }
-    });
-    __syncwarp();
-    int c = *w.count;
-    __syncwarp();
-    if (fill && c < a.select) {
-      // at most c of the first select + c tokens are not masked
-#pragma unroll 1
-      for (int v0 = 0; v0 < a.V && c < a.select; v0 += 32) {
-        const int v = v0 + lane;
-        const bool masked = v < a.V && mixed_logit<T>(logits, sh, v) == neg_inf();
-        const uint32_t take = __ballot_sync(kAllLanes, masked);
-        const int slot = c + __popc(take & ((1u << lane) - 1u));
-        if (masked) w.list[slot] = entry_key(none, v);  // slot < select + 32 <= kBeamListCap
-        c += __popc(take);
+        for (; reach != 0; reach &= reach - 1) {
+          const int slot = atomicAdd(w.count, 1);
+          if (slot < kBeamListCap) w.quarters[slot] = 4 * i + __ffs((int)reach) - 1;
+        }
       }
       __syncwarp();
+      n_list = *w.count;
+      __syncwarp();
     }
-    if (c >= a.select && c <= kBeamListCap) return c;
+    if (lane == 0) *w.count = 0;
+    __syncwarp();
+    if (n_list <= kBeamListCap) {
+      each_quarter<T, VEC>(a, logits, sh, w.quarters, n_list, [&](const float2(&x)[2], int q) {
+        uint32_t reach = (x[0].x < floor ? 0u : 1u) | (x[0].y < floor ? 0u : 2u) | (x[1].x < floor ? 0u : 4u) |
+                         (x[1].y < floor ? 0u : 8u);
+#pragma unroll 1
+        for (; reach != 0; reach &= reach - 1) {
+          const int j = __ffs((int)reach) - 1;
+          const float y = j & 2 ? (j & 1 ? x[1].y : x[1].x) : (j & 1 ? x[0].y : x[0].x);
+          const int slot = atomicAdd(w.count, 1);
+          const int token = (q >> 2) * kBeamGroup + quarter_offset<VEC>(q & 3, lane, j);
+          if (slot < kBeamListCap) w.list[slot] = entry_key(ordered_u32(y), token);
+        }
+      });
+      __syncwarp();
+      int c = *w.count;
+      __syncwarp();
+      if (c <= kBeamListCap) {
+        if (fill && c < a.select) {
+          // at most c of the first select + c tokens are not masked; other values may be rarer
+          const int end = rest == none ? a.V : min(a.V, kBeamFillTokens);
+#pragma unroll 1
+          for (int v0 = 0; v0 < end && c < a.select; v0 += 32) {
+            const int v = v0 + lane;
+            const bool equal = v < a.V && ordered_u32(mixed_logit<T>(logits, sh, v)) == rest;
+            const uint32_t take = __ballot_sync(kAllLanes, equal);
+            const int slot = c + __popc(take & ((1u << lane) - 1u));
+            if (equal) w.list[slot] = entry_key(rest, v);  // slot < select + 32 <= kBeamListCap
+            c += __popc(take);
+          }
+          __syncwarp();
+        }
+        if (c >= a.select) return c;
+        break;
+      }
+    }
+    if (fill || bound == 0xffffffffu) break;
+    fill = true;
+    rest = bound++;
   }
   row_best_exact<T>(a, logits, sh, tops, w);
   return a.select;
@@ -766,9 +780,10 @@ __device__ __noinline__ void finish_exact(const BeamSelectArgs& a, const FinishS
 // holds) the CTA counts exactly, beam by beam.
 //
 // About 7 us for 64 x 8 or 1 x 4 beams of 151936 logits: a chain of dependent loads (maxima,
-// bound, quarters), which more warps shorten.
+// bound, quarters), which more warps shorten.  A second CTA an SM would help many sequences
+// less than the registers that it takes hurt (64 x 1 beams 19.5 us with 64 of them, 18.0).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(32 * kBeamFinishWarps) beam_finish_kernel(BeamSelectArgs a) {
+__global__ void __launch_bounds__(32 * kBeamFinishWarps, 1) beam_finish_kernel(BeamSelectArgs a) {
   extern __shared__ __align__(16) char smem[];
   __shared__ int n_found, n_quarters;
   __shared__ uint32_t bound_key;

@@ -15,6 +15,7 @@ constexpr int kBeamScanCtas = 6;
 constexpr int kBeamFinishWarps = 16; // most warps of a sequence's finishing CTA
 constexpr int kBeamFinishCap = 256;  // quarter groups or candidates it lists before it counts exactly
 constexpr int kBeamListCap = 192;    // counting exactly: quarter groups or logits a warp lists
+constexpr int kBeamFillTokens = 2048; // tokens it searches for logits equal to the bound
 constexpr int kBeamRowScratch = kBeamListCap * 12 + 16;
 
 // One (value, token) entry of a row's list of best candidates.

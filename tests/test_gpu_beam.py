@@ -160,6 +160,35 @@ def test_select_many_of_a_small_vocabulary(cuda_device, dtype, n_seq, beams, sel
                                        finished.numpy(), 2))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [600, 5003, 20000])
+def test_select_many_equal_logits(cuda_device, dtype, V):
+    """More logits at one value than any list holds, few above it: everywhere, in the last tokens
+    only, mixed with lower ones, or at the type's lowest value."""
+    from dels_b200 import ops
+
+    dev = cuda_device
+    rng = np.random.default_rng(V)
+    x = torch.zeros(8, V)
+    x[1, : V - 400] = -3.0
+    x[2, ::2] = -1.0
+    x[3] = torch.finfo(dtype).min
+    x[4] = torch.from_numpy(np.sort(rng.integers(0, 3, V))).float()
+    x[5] = -0.0
+    x[6, : V - 300] = -INF
+    x[7] = float(torch.tensor(-1.17e-38).to(dtype))
+    for r in range(8):
+        x[r, torch.from_numpy(rng.permutation(V)[: 3 * (r % 4)])] = 2.0 + r
+    x = x.to(dtype)
+    cum = torch.from_numpy(rng.standard_normal((8, 1)).astype(np.float32))
+    for select in (1, 16, 64):
+        out = ops.beam_select(x.to(dev), cum.to(dev), select=select)
+        check_select(out, reference_select(np32(x), cum.numpy(), select))
+        both = ops.beam_select(x.to(dev), cum.view(4, 2).to(dev), select=select)
+        ref = reference_select(np32(x), cum.view(4, 2).numpy(), select)
+        np.testing.assert_allclose(both.scores.cpu().numpy(), ref[2], rtol=2e-7, atol=SCORE_TOL)
+
+
 @pytest.mark.parametrize("V", [1000, 1003])
 def test_select_scores_below_fp32(cuda_device, V):
     """Logits so far below the row's maximum that their scores fall to -inf: still the larger x
