@@ -49,29 +49,29 @@ def _reorder(kind, B, beams, select, width, length, heads, layers, inplace, name
 def listed():
     return [
         # the rank projection [256, 4096] of one hidden row: the smallest product of a draft step
-        _linear(1, 4096, 256, "bf16", False, "rank projection 1 row"),
+        _linear(1, 4096, 256, "bf16", False, "rank projection, 1 row"),
         # the long logits of one sequence's draft block: streams the whole LM head
-        _linear(16, 4096, _VOCAB, "bf16", False, "lm head 16 rows"),
+        _linear(16, 4096, _VOCAB, "bf16", False, "lm head, 16 rows"),
         # the long logits of 32 sequences x 16 positions: bound by the tensor cores
-        _linear(512, 4096, _VOCAB, "bf16", False, "lm head 512 rows"),
+        _linear(512, 4096, _VOCAB, "bf16", False, "lm head, 512 rows"),
         # a biased fp32 layer whose sizes divide nothing
-        _linear(77, 2561, 1003, "f32", True, "odd sizes fp32"),
+        _linear(77, 2561, 1003, "f32", True, "odd sizes, fp32"),
         # one sequence, four beams, one draft step: latency counts
-        _select(1, 4, 4, _VOCAB, "bf16", True, "none", False, "select 1 x 4 beams"),
+        _select(1, 4, 4, _VOCAB, "bf16", True, "none", False, "select, 1 x 4 beams"),
         # a full serving batch of the same step
-        _select(64, 8, 8, _VOCAB, "bf16", True, "none", False, "select 64 x 8 beams"),
+        _select(64, 8, 8, _VOCAB, "bf16", True, "none", False, "select, 64 x 8 beams"),
         # constrained decoding in fp32: a few allowed tokens, rows without any, finished beams, odd vocabulary
-        _select(5, 3, 6, 32003, "f32", False, "few", True, "select masked fp32"),
+        _select(5, 3, 6, 32003, "f32", False, "few", True, "select, masked fp32"),
         # the first step: one root per sequence opens 16 beams, half of the vocabulary masked
-        _select(64, 1, 16, _VOCAB, "bf16", False, "half", False, "select first step"),
+        _select(64, 1, 16, _VOCAB, "bf16", False, "half", False, "select, first step"),
         # one sequence's GRU state and token history
-        _reorder("gru", 1, 4, 4, 1024, 14, 1, 1, False, "reorder 1 x 4 beams"),
+        _reorder("gru", 1, 4, 4, 1024, 14, 1, 1, False, "reorder, 1 x 4 beams"),
         # the same for a full serving batch
-        _reorder("gru", 64, 8, 8, 1024, 14, 1, 1, False, "reorder 64 x 8 beams"),
+        _reorder("gru", 64, 8, 8, 1024, 14, 1, 1, False, "reorder, 64 x 8 beams"),
         # two layers of a key and value cache, the used part of a longer allocation, in place
-        _reorder("cache", 4, 8, 8, 128, 1537, 8, 2, True, "reorder kv cache"),
+        _reorder("cache", 4, 8, 8, 128, 1537, 8, 2, True, "reorder, kv cache"),
         # beams opening from three to five, rows of an odd number of bytes
-        _reorder("bytes", 7, 3, 5, 4099, 1, 1, 1, False, "reorder odd bytes"),
+        _reorder("bytes", 7, 3, 5, 4099, 1, 1, 1, False, "reorder, odd bytes"),
     ]
 
 
