@@ -348,8 +348,10 @@ DELS_API int dels_correction_mid_tc_bf16(const void* h, int64_t ld_h, const void
  * reference): the LM head and the projections at half the bytes and twice the tensor rate
  * of bf16.
  *   dels_quantize_rows_i8   a = max |x[i]|, scale[i] = a / 127,
- *                           q[i, k] = rint(x[i, k] * (127 / a)), half to even, in fp32;
- *                           weights [N, K] once (a scale per channel), activations per call.
+ *                           q[i, k] = rint(x[i, k] * (127 / a)), half to even, in fp32
+ *                           with each operation rounded (127 / a of fp32 rows is
+ *                           127 * (1 / a), as tensor expressions evaluate it); weights
+ *                           [N, K] once (a scale per channel), activations per call.
  *                           A zero row gives scale 0; NaN or infinity in a row gives that
  *                           scale and q = 0, so its products are NaN.
  *   dels_linear_i8          out[i, n] = (sum_k xq[i, k] wq[n, k]) * x_scale[i] * w_scale[n]
