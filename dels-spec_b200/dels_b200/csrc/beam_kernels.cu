@@ -952,7 +952,9 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps, 1) beam_finish_kernel(B
     }
   }
   __syncthreads();
-  if (fill && n_found < n) {
+  int c = n_found;
+  if (fill && c < n) {
+    __syncthreads();  // all threads have taken this branch by the count that warp 0 now changes
     // The rest are masked tokens, the lowest of the lowest beam.  A beam whose own score is
     // not finite, or whose lowest logits fall out of fp32 below its maximum, has other candidates
     // at -inf, which an exact count sorts out.
@@ -961,7 +963,6 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps, 1) beam_finish_kernel(B
     if (warp == 0 && row_score(-3.402823466e+38f, f.stat[0]) > neg_inf() && f.stat[0].y < -neg_inf()) {
       const Shared<T> sh = shared_terms<T>(a, seq);
       const T* logits = static_cast<const T*>(a.logits) + (long long)row * a.ld;
-      int c = n_found;
 #pragma unroll 1
       for (int v0 = 0; v0 < a.V && c < n; v0 += 32) {
         const int v = v0 + lane;
@@ -975,8 +976,8 @@ __global__ void __launch_bounds__(32 * kBeamFinishWarps, 1) beam_finish_kernel(B
       if (lane == 0) n_found = c;
     }
     __syncthreads();
+    c = n_found;
   }
-  const int c = n_found;
   if (exact || n_quarters > kBeamFinishCap || c < n || c > kBeamFinishCap) {
     finish_exact<T, VEC>(a, f);
     return;
