@@ -45,6 +45,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "dels_last_error": (ctypes.c_char_p, []),
     "dels_init": (_I, [_I]),
     "dels_sm_count": (_I, [_I]),
+    "dels_stream_capture_id": (ctypes.c_uint64, [_P]),
     "dels_rank_workspace_bytes": (_SZ, [_I, _I, _I]),
     "dels_rank_project_bf16": (
         _I,

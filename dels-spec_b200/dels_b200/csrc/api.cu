@@ -1054,6 +1054,16 @@ int dels_sm_count(int device) {
   return g_dev[device].sm_count;
 }
 
+uint64_t dels_stream_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 size_t dels_rank_workspace_bytes(int rows, int K, int r) {
   if (rows <= 0 || K <= 0 || r <= 0) return DELS_WS_HEADER_BYTES;
   return DELS_WS_HEADER_BYTES + projection_partials_bytes(rows, K, r);

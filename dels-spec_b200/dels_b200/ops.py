@@ -117,11 +117,37 @@ class Workspace:
 
 
 _ws_cache: dict[tuple[int, int], Workspace] = {}
+_capture_ws: dict[tuple[int, int], tuple[int, Workspace]] = {}
+
+
+def _capture_id(stream: int) -> int:
+    """The number of the graph capture that the current stream, ``stream``, is part of; 0 outside one."""
+    if not torch._C._cuda_isCurrentStreamCapturing():
+        return 0
+    return int(_lib.query("dels_stream_capture_id", stream))
 
 
 def workspace(nbytes: int, device: torch.device) -> Workspace:
-    """A cached workspace per (device, stream) large enough for ``nbytes``."""
-    key = (device.index or 0, torch.cuda.current_stream(device).cuda_stream)
+    """A cached workspace per (device, stream) large enough for ``nbytes``.
+
+    A graph keeps the addresses that its capture saw, so a capture shares no workspace with
+    calls outside it or with another capture (``torch.cuda.graph`` captures on one stream by
+    default): it gets one of its own, in the graph's memory pool."""
+    return _stream_workspace(nbytes, device, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _stream_workspace(nbytes: int, device: torch.device, stream: int) -> Workspace:
+    """workspace() for a stream that is known already."""
+    key = (device.index or 0, stream)
+    capture = _capture_id(stream)
+    if capture:
+        # a larger one for a later call of the same capture: the pool gives the smaller one's memory
+        # to what the capture allocates after it, which runs after it
+        last, ws = _capture_ws.get(key, (0, None))
+        if last != capture or ws.nbytes < nbytes:
+            ws = Workspace(max(nbytes, 1 << 20), device)
+            _capture_ws[key] = (capture, ws)
+        return ws
     ws = _ws_cache.get(key)
     if ws is None or ws.nbytes < nbytes:
         ws = Workspace(max(nbytes, 1 << 20), device)
@@ -899,12 +925,6 @@ def _raw_stream(device: torch.device) -> int:
 @functools.lru_cache(maxsize=4096)
 def _bytes(query: str, *args: int) -> int:
     return int(_lib.query(query, *args))
-
-
-def _stream_workspace(nbytes: int, device: torch.device, stream: int) -> Workspace:
-    """workspace() for a stream that is known already."""
-    ws = _ws_cache.get((device.index, stream))
-    return workspace(nbytes, device) if ws is None or ws.nbytes < nbytes else ws
 
 
 def quantize_rows_i8(

@@ -71,6 +71,11 @@ DELS_API int dels_init(int device);
 /* Number of streaming multiprocessors the persistent kernels size their grids for. */
 DELS_API int dels_sm_count(int device);
 
+/* The number of the graph capture that `stream` is part of, 0 outside one.  A graph keeps
+ * the workspace address that its capture saw: a host that caches workspaces gives every
+ * capture one of its own and keeps it as long as the graph. */
+DELS_API uint64_t dels_stream_capture_id(void* stream);
+
 /* ---------------------------------------------------------------------------------
  * Rank projection.  Replaces code/kernel/dels.py:437-439
  *   rank_state = F.linear(h, W_rank); rank_state = F.silu(rank_state) (optional)
