@@ -70,6 +70,16 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
+// a b + c of packed fp32, each rounded once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+
 // (m, s) of two parts of a softmax; s counts exp(x - m).
 __device__ __forceinline__ float2 softmax_join(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x);
@@ -206,15 +216,25 @@ __device__ __forceinline__ void load_single(const T* const (&row)[2], const Shar
   }
 }
 
-// Takes a lane's logits of a group of N rows into their running softmax (m, the same in all
-// lanes, and the lane's own sums s); t: the maxima of the quarters, NaN where one holds it,
-// and then the sums are NaN.  Two rows at a time fill each other's waits.
-template <int N>
-__device__ __forceinline__ void fold_group(const float2 (&x)[N][kPer / 2], float (&m)[N], float2 (&s)[N],
-                                           float4 (&t)[N]) {
-  float nref[N];
+// The softmax of a warp's two rows as its run over them goes on.  nref: minus the reference of the
+// exponentials (0 before there is one), the same in all lanes; (s.x, s.y): the lane's own sums of
+// exp(x + nref) of the two, (less.x, less.y): what their rounding left out, to be added; m: lane
+// r's maximum of row r.  A reference follows its maximum only when that passes `limit`, kLag above
+// the reference: a row that climbs a little in every group would else be rounded by a rescaling in
+// each.
+struct RowSoftmax {
+  float m, nref[2], limit[2];
+  float2 s, less;
+};
+constexpr float kLag = 16.0f;
+
+// Takes a lane's logits of a group of two rows into their running softmax; t: the maxima of the
+// quarters, NaN where one holds it, and then the sums are NaN.  Two rows at a time fill each
+// other's waits.  A group's terms are added in pairs and then, compensated, to the sum: one by one
+// they rounded the same way, 5e-5 of a sum over 524288 equal logits.
+__device__ __forceinline__ void fold_group(const float2 (&x)[2][kPer / 2], int lane, RowSoftmax& w, float4 (&t)[2]) {
 #pragma unroll
-  for (int r = 0; r < N; ++r) {
+  for (int r = 0; r < 2; ++r) {
     float q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -224,23 +244,36 @@ __device__ __forceinline__ void fold_group(const float2 (&x)[N][kPer / 2], float
     t[r] = make_float4(q[0], q[1], q[2], q[3]);
   }
 #pragma unroll
-  for (int r = 0; r < N; ++r) {
+  for (int r = 0; r < 2; ++r) {
     const float top = fmax3_nan(fmax_nan(t[r].x, t[r].y), t[r].z, t[r].w);
-    if (top > m[r]) {
-      const float down = __expf(m[r] - top);  // m = -inf: the sums are 0 and stay 0
-      s[r] = mul2(s[r], make_float2(down, down));
-      m[r] = top;
+    if (lane == r) w.m = fmaxf(w.m, top);
+    if (top > w.limit[r]) {
+      const float down = w.limit[r] == neg_inf() ? 0.0f : expf(-w.nref[r] - top);  // (the first one's sums are 0)
+      const float2 by = r == 0 ? make_float2(down, 1.0f) : make_float2(1.0f, down);
+      w.s = mul2(w.s, by);
+      w.less = mul2(w.less, by);
+      w.nref[r] = -top;
+      w.limit[r] = top + kLag;
     }
-    nref[r] = m[r] == neg_inf() ? 0.0f : -m[r];
   }
+  float2 e[2][kPer / 2];
 #pragma unroll
   for (int i = 0; i < kPer / 2; ++i)
 #pragma unroll
-    for (int r = 0; r < N; ++r) {
-      const float2 e =
-          mul2(add2(x[r][i], make_float2(nref[r], nref[r])), make_float2(1.4426950408889634f, 1.4426950408889634f));
-      s[r] = add2(s[r], make_float2(exp2_approx(e.x), exp2_approx(e.y)));
+    for (int r = 0; r < 2; ++r) {
+      const float2 y =
+          mul2(add2(x[r][i], make_float2(w.nref[r], w.nref[r])), make_float2(1.4426950408889634f, 1.4426950408889634f));
+      e[r][i] = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+      // a pair is added as soon as both of its sums are there
+#pragma unroll
+      for (int o = 1; o < kPer / 2; o *= 2)
+        if ((i & (2 * o - 1)) == 2 * o - 1) e[r][i] = add2(e[r][i - o], e[r][i]);
     }
+  constexpr int last = kPer / 2 - 1;
+  const float2 y = add2(make_float2(e[0][last].x + e[0][last].y, e[1][last].x + e[1][last].y), w.less);
+  const float2 sum = add2(w.s, y);
+  w.less = add2(y, fma2(sum, make_float2(-1.0f, -1.0f), w.s));
+  w.s = sum;
 }
 
 }  // namespace
@@ -308,14 +341,11 @@ __global__ void __launch_bounds__(32 * kBeamScanWarps, kBeamScanCtas) beam_scan_
     }
     const int n_mine = min(N, n_live - N * pair);  // rows of this warp, from the N pair-th on
     const Shared<T> sh = shared_terms<T>(a, run);  // (without shared terms there is one run)
-    float m[N];
-    float2 s[N];
+    RowSoftmax w = {neg_inf(), {0.0f, 0.0f}, {neg_inf(), neg_inf()}, {0.0f, 0.0f}, {0.0f, 0.0f}};
     float4* tops[N];
     const T* row[N];
 #pragma unroll
     for (int r = 0; r < N; ++r) {
-      m[r] = neg_inf();
-      s[r] = make_float2(0.0f, 0.0f);
       const int k = __shfl_sync(kAllLanes, my_row, min(N * pair + r, n_live - 1));
       tops[r] = a.ws.group_top + (long long)(row0 + k) * a.groups;
       row[r] = logits + k * a.ld;
@@ -395,7 +425,7 @@ __global__ void __launch_bounds__(32 * kBeamScanWarps, kBeamScanCtas) beam_scan_
         load_single<T>(row, sh, g * kBeamGroup, a.V, lane, x);
       }
       float4 t[N];
-      fold_group<N>(x, m, s, t);
+      fold_group(x, lane, w, t);
 #pragma unroll
       for (int r = 0; r < N; ++r)
         if (lane == r && r < n_mine) tops[r][g] = t[r];
@@ -403,10 +433,13 @@ __global__ void __launch_bounds__(32 * kBeamScanWarps, kBeamScanCtas) beam_scan_
     __syncthreads();  // the block before has been joined, and all slots are read
 #pragma unroll
     for (int r = 0; r < N; ++r) {
-      float sum = s[r].x + s[r].y;
+      float sum = r == 0 ? w.s.x + w.less.x : w.s.y + w.less.y;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAllLanes, sum, o);
-      if (lane == 0 && r < n_mine) team_part[team][N * pair + r] = make_float2(m[r], sum);
+      // (without a reference there is nothing to rescale: m = -inf and a sum of 0, or NaN)
+      if (lane == r && r < n_mine)
+        team_part[team][N * pair + r] =
+            make_float2(w.m, w.limit[r] == neg_inf() || w.m == -w.nref[r] ? sum : sum * expf(-w.nref[r] - w.m));
     }
     __syncthreads();
     if (warp == 0 && lane < n_live) {
