@@ -107,6 +107,12 @@ __host__ __device__ constexpr uint32_t make_idesc_s8_s32(int M, int N) {
          | ((uint32_t)(M >> 4) << 24);    // M / 16
 }
 
+// A result from its integer sum: two roundings of the product, the second with the bias (0 where
+// there is none), the same in every kernel, so that a row's results do not depend on its company.
+__device__ __forceinline__ float i8_result(int sum, float sx, float sw, float bias) {
+  return __fmaf_rn(__fmul_rn(__int2float_rn(sum), sx), sw, bias);
+}
+
 // One channel's results for the COLS rows row0.. of a tile; `valid` of them exist, the others
 // are computed all the same and not stored, so that no branch keeps the rows' chains apart.
 template <int COLS, typename OutT>
@@ -119,8 +125,8 @@ __device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float*
       const bool odd = lane & 1;
 #pragma unroll
       for (int j = 0; j < COLS; j += 2) {
-        const float y0 = __int2float_rn((int)v[j]) * scale[j] * sw + bias;
-        const float y1 = __int2float_rn((int)v[j + 1]) * scale[j + 1] * sw + bias;
+        const float y0 = i8_result((int)v[j], scale[j], sw, bias);
+        const float y1 = i8_result((int)v[j + 1], scale[j + 1], sw, bias);
         const float other = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 1);
         const uint32_t pair = odd ? pack_bf16x2(other, y1) : pack_bf16x2(y0, other);
         if (channel_ok && j + (int)odd < valid)
@@ -131,7 +137,7 @@ __device__ __forceinline__ void i8_store(const uint32_t (&v)[COLS], const float*
   }
 #pragma unroll
   for (int j = 0; j < COLS; ++j) {
-    const float y = __int2float_rn((int)v[j]) * scale[j] * sw + bias;
+    const float y = i8_result((int)v[j], scale[j], sw, bias);
     if (channel_ok && j < valid) {
       if constexpr (sizeof(OutT) == 2)
         out[j * ld] = __float2bfloat16_rn(y);

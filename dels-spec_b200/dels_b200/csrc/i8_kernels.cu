@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(kI8GemvThreads, kI8GemvCtas) i8_gemv_kernel(I8
       }
     const int r = lane / G, channel = n + lane % G;
     if (r < a.rows && channel < a.n_out) {
-      float y = __int2float_rn(mine) * scale[r] * a.sw[channel];
-      if (a.bias != nullptr) y += to_f32(static_cast<const OutT*>(a.bias)[channel]);
+      const float bias = a.bias != nullptr ? to_f32(static_cast<const OutT*>(a.bias)[channel]) : 0.0f;
+      const float y = i8_result(mine, scale[r], a.sw[channel], bias);
       OutT* out = static_cast<OutT*>(a.out) + (long long)r * a.ld_out + channel;
       if constexpr (sizeof(OutT) == 2)
         *out = __float2bfloat16_rn(y);

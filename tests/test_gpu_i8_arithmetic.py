@@ -70,3 +70,28 @@ def test_fp32_rows_of_extreme_magnitude(cuda_device):
     for e in (-110, -100, 60, 105, 124):  # (the smallest values stay normal numbers)
         dx = torch.from_numpy(np.ldexp(x, e).astype(np.float32)).to(dev)
         np.testing.assert_array_equal(ops.quantize_rows_i8(dx)[0].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("biased", [True, False])
+def test_a_row_gives_the_same_bits_in_any_call(cuda_device, dtype, biased):
+    """A row's products do not depend on how many rows come with it: one and two rows, a tile of them,
+    pairs of tiles; scales of both signs and a channel of zeros with a negative one among the weights."""
+    from dels_b200 import ops
+
+    dev = cuda_device
+    K, N = 300, 30011
+    g = torch.Generator(device=dev).manual_seed(9)
+    x = torch.randn(300, K, generator=g, device=dev).to(dtype)
+    wq, sw = ops.quantize_rows_i8(torch.randn(N, K, generator=g, device=dev))
+    wq[6] = 0
+    sw[::3] *= -1
+    bias = torch.randn(N, generator=g, device=dev).to(dtype) if biased else None
+    whole = ops.linear_w8a8(x, wq, sw, bias)
+    bits = torch.int32 if dtype == torch.float32 else torch.int16
+    for rows in (1, 2, 3, 40, 129):
+        part = ops.linear_w8a8(x[:rows], wq, sw, bias)
+        assert torch.equal(part.view(bits), whole[:rows].view(bits)), rows
+        # and from rows that were quantised before
+        q, s = ops.quantize_rows_i8(x[:rows])
+        assert torch.equal(ops.linear_i8(q, s, wq, sw, bias, out_dtype=dtype).view(bits), part.view(bits)), rows
