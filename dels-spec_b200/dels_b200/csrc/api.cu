@@ -723,6 +723,12 @@ int fused_argmax_common(const void* h, long long ld_h, const void* W, long long 
   return launch_tc<256, kArgmax, false>(op, a, ds->sm_count, st);
 }
 
+// The sizes that a selection takes; groups of all rows are counted in 32 bits.
+bool beam_select_takes(int n_seq, int beams, int select, int V) {
+  return n_seq >= 0 && beams >= 1 && beams <= kBeamMax && select >= 1 && select <= kBeamMax && V >= select &&
+         V <= DELS_BEAM_MAX_VOCAB && (long long)n_seq * beams <= (1ll << 20);
+}
+
 // Plans a selection's scan and lays out its scratch over `base` (counted only when `a` is
 // null); returns the scratch's bytes.
 size_t beam_plan(int n_seq, int beams, int V, int elem, bool shared, int sm_count, char* base, BeamSelectArgs* a) {
@@ -1702,7 +1708,7 @@ int dels_gather_scaled_rows_bf16(const int64_t* tokens, int64_t tok_stride, int 
 }
 
 size_t dels_beam_select_workspace_bytes(int n_seq, int beams, int select, int V) {
-  if (n_seq <= 0 || beams <= 0 || select <= 0 || V <= 0) return DELS_WS_HEADER_BYTES;
+  if (n_seq == 0 || !beam_select_takes(n_seq, beams, select, V)) return DELS_WS_HEADER_BYTES;
   // whatever the device, the type and whether logits are shared
   size_t most = 0;
   for (int i = 0; i < 4; ++i) {
@@ -1722,7 +1728,7 @@ int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const voi
     return fail(DELS_ERR_INVALID_ARG, "beams and select must be in 1..%d (got %d, %d)", kBeamMax, beams, select);
   if (V < select || V > DELS_BEAM_MAX_VOCAB)
     return fail(DELS_ERR_INVALID_ARG, "V must be in select..%d (got %d, select %d)", DELS_BEAM_MAX_VOCAB, V, select);
-  if ((long long)n_seq * beams > (1ll << 20))  // groups of all rows are counted in 32 bits
+  if (!beam_select_takes(n_seq, beams, select, V))
     return fail(DELS_ERR_INVALID_ARG, "at most 2^20 rows (got %lld)", (long long)n_seq * beams);
   if (dtype != DELS_DTYPE_BF16 && dtype != DELS_DTYPE_F32) return fail(DELS_ERR_INVALID_ARG, "unknown dtype %d", dtype);
   const size_t elem = dtype == DELS_DTYPE_BF16 ? 2 : 4;
