@@ -96,6 +96,7 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
   } while (0)
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
@@ -827,6 +828,12 @@ int check_i8_matrix(const char* name, const void* p, long long ld, long long k) 
   if (!aligned16(p)) return fail(DELS_ERR_ALIGNMENT, "%s must be 16-byte aligned", name);
   if (ld < k || (ld % 16) != 0)
     return fail(DELS_ERR_ALIGNMENT, "%s: leading dimension %lld must be >= %lld and a multiple of 16", name, ld, k);
+  return DELS_OK;
+}
+
+int check_i8_scale(const char* name, const float* p) {
+  if (p == nullptr) return fail(DELS_ERR_INVALID_ARG, "%s is NULL", name);
+  if (!aligned_to(p, 4)) return fail(DELS_ERR_ALIGNMENT, "%s must be aligned to its elements", name);
   return DELS_OK;
 }
 
@@ -1741,6 +1748,9 @@ int dels_beam_select(const void* logits, int dtype, int64_t ld_logits, const voi
     return fail(DELS_ERR_INVALID_ARG, "pad_token %d outside the vocabulary of %d", pad_token, V);
   if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(base)) % elem != 0)
     return fail(DELS_ERR_ALIGNMENT, "logits and base must be aligned to their elements");
+  if (!aligned_to(prior, 4) || !aligned_to(beta, 4) || !aligned_to(cum, 4) || !aligned_to(parents, 4) ||
+      !aligned_to(tokens, 8) || !aligned_to(scores, 4))
+    return fail(DELS_ERR_ALIGNMENT, "prior, beta, cum, parents, tokens and scores must be aligned to their elements");
   WsHeader hdr;
   if ((rc = ws_header(ws, ws_bytes, dels_beam_select_workspace_bytes(n_seq, beams, select, V), &hdr)) != DELS_OK)
     return rc;
@@ -1784,6 +1794,8 @@ int dels_beam_reorder(const dels_beam_state* states_in, int n_states, const int3
     return fail(DELS_ERR_INVALID_ARG, "beams and select must be in 1..%d (got %d, %d)", kBeamMax, beams, select);
   if (n_states > 0 && (states_in == nullptr || (parents == nullptr && n_seq > 0)))
     return fail(DELS_ERR_INVALID_ARG, "NULL argument");
+  if (!aligned_to(parents, 4) || !aligned_to(status, 4))
+    return fail(DELS_ERR_ALIGNMENT, "parents and status must be aligned to their elements");
   for (int i = 0; i < n_states; ++i)
     if ((rc = check_beam_state(states_in[i], i, n_seq, beams, select)) != DELS_OK) return rc;
   DeviceState* ds = nullptr;
@@ -1826,6 +1838,7 @@ int dels_quantize_rows_i8(const void* x, int dtype, int64_t ld_x, int rows, int 
   int rc;
   if ((rc = check_quantize(x, dtype, ld_x, rows, K)) != DELS_OK) return rc;
   if (rows > 0 && scale == nullptr) return fail(DELS_ERR_INVALID_ARG, "scale is NULL");
+  if (!aligned_to(scale, 4)) return fail(DELS_ERR_ALIGNMENT, "scale must be aligned to its elements");
   if (rows > 0 && (rc = check_i8_matrix("q", q, ld_q, K)) != DELS_OK) return rc;
   DeviceState* ds = nullptr;
   if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
@@ -1842,10 +1855,10 @@ int dels_linear_i8(const int8_t* xq, int64_t ld_xq, const float* x_scale, const 
   if (rows > 0) {
     if ((rc = check_i8_matrix("xq", xq, ld_xq, K)) != DELS_OK) return rc;
     if ((rc = check_i8_out(out, out_dtype, ld_out, bias, N)) != DELS_OK) return rc;
-    if (x_scale == nullptr) return fail(DELS_ERR_INVALID_ARG, "x_scale is NULL");
+    if ((rc = check_i8_scale("x_scale", x_scale)) != DELS_OK) return rc;
   }
   if ((rc = check_i8_matrix("wq", wq, ld_wq, K)) != DELS_OK) return rc;
-  if (w_scale == nullptr) return fail(DELS_ERR_INVALID_ARG, "w_scale is NULL");
+  if ((rc = check_i8_scale("w_scale", w_scale)) != DELS_OK) return rc;
   WsHeader hdr;
   if ((rc = ws_header(ws, ws_bytes, DELS_WS_HEADER_BYTES, &hdr)) != DELS_OK) return rc;
   DeviceState* ds = nullptr;
@@ -1869,15 +1882,17 @@ int dels_linear_w8a8(const void* x, int x_dtype, int64_t ld_x, const int8_t* wq,
                      size_t ws_bytes, void* stream) {
   int rc;
   if ((rc = check_i8_shape(rows, K, N)) != DELS_OK) return rc;
-  if (rows > 0 && (rc = check_i8_out(out, out_dtype, ld_out, bias, N)) != DELS_OK) return rc;
+  if (rows > 0) {
+    if ((rc = check_quantize(x, x_dtype, ld_x, rows, K)) != DELS_OK) return rc;
+    if ((rc = check_i8_out(out, out_dtype, ld_out, bias, N)) != DELS_OK) return rc;
+  }
   if ((rc = check_i8_matrix("wq", wq, ld_wq, K)) != DELS_OK) return rc;
-  if (w_scale == nullptr) return fail(DELS_ERR_INVALID_ARG, "w_scale is NULL");
+  if ((rc = check_i8_scale("w_scale", w_scale)) != DELS_OK) return rc;
   WsHeader hdr;
   if ((rc = ws_header(ws, ws_bytes, dels_linear_w8a8_workspace_bytes(rows, K), &hdr)) != DELS_OK) return rc;
   DeviceState* ds = nullptr;
   if ((rc = current_device_state(&ds)) != DELS_OK) return rc;
   if (rows > 0 && i8_few_rows(rows, K, N)) {
-    if ((rc = check_quantize(x, x_dtype, ld_x, rows, K)) != DELS_OK) return rc;
     const bool vec = aligned16(x) && (ld_x * (x_dtype == DELS_DTYPE_BF16 ? 2 : 4)) % 16 == 0;
     return launch_i8_gemv({x, ld_x, vec, nullptr, wq, ld_wq, w_scale, bias, out, ld_out, rows, K, N},
                           x_dtype == DELS_DTYPE_BF16 ? kI8FromBf16 : kI8FromF32, out_dtype == DELS_DTYPE_BF16,
