@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from dataclasses import dataclass
 
 import torch
@@ -1015,7 +1016,21 @@ def linear_w8a8(
     """F.linear(x, W, bias) with W = wq * w_scale[:, None] and every row of ``x`` (bf16 or
     fp32) quantised on the way: quantize_rows_i8 and linear_i8 in one call, the weights
     loading while the rows are quantised.  The result has x's type unless ``out`` or
-    ``out_dtype`` says otherwise."""
+    ``out_dtype`` says otherwise.  ``x`` [..., K] gives [..., N]; rows that are not evenly
+    spaced (a slice of [B, S, K] along S) are copied first."""
+    if isinstance(x, torch.Tensor) and x.dim() != 2 and x.dim() > 0:
+        *lead, K = x.shape
+        rows, flat = math.prod(lead), None
+        if out is not None:
+            _require_float("out", out, x.dim())
+            if list(out.shape[:-1]) != lead:
+                raise ValueError(f"out {tuple(out.shape)} does not match x {tuple(x.shape)}")
+            try:
+                flat = out.view(rows, out.shape[-1])
+            except RuntimeError:
+                raise ValueError(f"out's rows must be evenly spaced (stride {out.stride()})") from None
+        y = linear_w8a8(x.reshape(rows, K), wq, w_scale, bias, out=flat, out_dtype=out_dtype, ws=ws)
+        return y.view(*lead, y.shape[1]) if out is None else out
     code = _require_float("x", x, 2)
     dev = x.device
     rows, K = x.shape
