@@ -777,8 +777,8 @@ int launch_beam_select(BeamSelectArgs a, bool bf16, bool shared, bool vec, cudaS
   // instead of 56.
   a.finish_direct = 4ll * a.groups * a.beams < 2ll * a.select;
   // Warps that share a beam: enough for every group, or quarter, to be loaded at once, up to
-  // sixteen for all beams (1 x 4 beams of 151936 logits 11.4 us, 13.3 with a warp for each beam;
-  // 64 x 8 beams 48.7 and 51.0).  More would offer nothing but what they do not have.
+  // sixteen for all beams (of 151936 logits without shared ones, 1 x 4 beams 11.4 us, 13.3 with a
+  // warp for each beam; 64 x 8 beams 48.7 and 51.0).  More would offer nothing but what they do not have.
   const int parts = a.finish_direct ? 4 * a.groups : cdiv(a.groups, 32);
   int split = 1;
   while (split < parts && 2 * split * a.beams <= kBeamFinishWarps) split *= 2;

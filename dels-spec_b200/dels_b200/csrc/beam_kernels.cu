@@ -286,13 +286,13 @@ __device__ __forceinline__ void fold_group(const float2 (&x)[2][kPer / 2], int l
 // the block].  With VEC a team has the next groups copied into its ring in shared memory ahead
 // of its arithmetic (bulk copies: no registers held, a handful of instructions a group).
 //
-// 64 x 8 beams of 151936 bf16 logits with shared ones, 175 MB: 47 us, 3.7 TB/s.  No unit is
-// full (ALU and FMA pipes 40 %, special functions 45 %, 0.63 instructions a cycle of each
-// scheduler): 394 instructions a warp and group, of which 32 are exponentials and 8 warp
+// 64 x 8 beams of 151936 bf16 logits with shared ones, 175 MB: 49 us, 3.6 TB/s.  No unit is
+// full (ALU pipe 39 %, FMA 37 %, special functions 41 %, 0.61 instructions a cycle of each
+// scheduler): 398 instructions a warp and group, of which 32 are exponentials and 8 warp
 // reductions, wait for one another, and 24 warps an SM hide a part of it.  Rows that cannot be
 // copied (VEC false: 16-byte alignment, V a multiple of 8) are loaded a group at once instead:
-// 64 x 8 beams without shared logits 60 us at an odd address, 49 us aligned; 1 x 4 beams 15.3
-// and 11.4 us.
+// 64 x 8 beams without shared logits 63 us at an odd address, 48 us aligned; 1 x 4 beams 15.6
+// and 11.2 us.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kBeamScanWarps, kBeamScanCtas) beam_scan_kernel(BeamSelectArgs a) {
   constexpr int D = beam_scan_depth(sizeof(T));
@@ -644,7 +644,7 @@ __device__ __forceinline__ int row_best(const BeamSelectArgs& a, const T* logits
   // With too little above -inf: all that is, and the lowest masked tokens.  Where more logits than
   // the list holds reach the bound, many of them mostly equal it (a mask of the type's lowest value,
   // constant rows): those above it, and the lowest tokens of the rest, 64 x 1 beams that take 16 with
-  // one token allowed 59 us instead of 618.
+  // one token allowed 65 us instead of 618.
   bool fill = bound <= none;
   if (fill) bound = none + 1;
 #pragma unroll 1
@@ -814,7 +814,7 @@ __device__ __noinline__ void finish_exact(const BeamSelectArgs& a, const FinishS
 //
 // About 7 us for 64 x 8 or 1 x 4 beams of 151936 logits: a chain of dependent loads (maxima,
 // bound, quarters), which more warps shorten.  A second CTA an SM would help many sequences
-// less than the registers that it takes hurt (64 x 1 beams 19.5 us with 64 of them, 18.0).
+// less than the registers that it takes hurt (64 x 1 beams 1.5 us longer with 64 of them).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kBeamFinishWarps, 1) beam_finish_kernel(BeamSelectArgs a) {
   extern __shared__ __align__(16) char smem[];
@@ -1052,9 +1052,10 @@ BeamKernel beam_finish_kernel_for(bool bf16, bool vec) {
 // and what is written to an aligned address is put together from five 32-bit words where
 // source and destination differ modulo 16.
 //
-// Bound by memory: 617 MB read and written of a cache in place take 97 us, 6.3 TB/s, what a
-// plain copy does; 64 x 8 GRU states of 2 KB and their histories 3.4 us, rows of 4099 bytes
-// 3.9 us (13.3 when they moved by bytes), which is a launch and three passes of latency.
+// Bound by memory: a cache of 8 beams in place, of which 597 MB have to be read and written for
+// random parents (a row that keeps its place is neither), 98 us, 6.1 TB/s, 0.94 of a plain copy's
+// rate; 64 x 8 GRU states of 2 KB and their histories 3.4 us, rows of 4099 bytes 3.8 us (13.3 when
+// they moved by bytes), which is a launch and three passes of latency.
 // --------------------------------------------------------------------------------
 namespace {
 

@@ -10,7 +10,8 @@ constexpr int kBeamMax = 64;         // beams of a sequence, read or selected
 constexpr int kBeamGroup = 512;      // logits of a group, the unit a warp scans at a time
 constexpr int kBeamScanWarps = 4;    // most warps of a scanning CTA
 constexpr int kBeamScanRows = 8;     // most rows a scanning CTA takes together
-// Most scanning CTAs of an SM: 64 x 8 beams 53 us (5: 60, 7 with a shorter ring: 53, 8: 54).
+// Most scanning CTAs of an SM.  64 x 8 beams took 53 us when this was chosen (5: 60, 7 with a
+// shorter ring: 53, 8: 54); compensated sums have made that 55.
 constexpr int kBeamScanCtas = 6;
 constexpr int kBeamFinishWarps = 16; // most warps of a sequence's finishing CTA
 constexpr int kBeamFinishCap = 256;  // quarter groups or candidates it lists before it counts exactly
@@ -111,7 +112,7 @@ struct BeamState {
   long long tile0;   // first tile of this state
 };
 
-// States of a launch.  Their 2.3 KB of arguments cost nothing that shows: a list of at most four
+// States of a launch.  Their 2.5 KB of arguments cost nothing that shows: a list of at most four
 // took 3.4 us on the device and 3.7 us of the host's time for two states, as this one does.
 constexpr int kBeamStatesPerLaunch = 32;
 constexpr int kBeamThreads = 256;
@@ -129,7 +130,7 @@ struct BeamStates {
 
 // A tile's stage: each beam's piece, up to 15 bytes before it and a word after.
 constexpr int kBeamReorderSmem = 33792;
-constexpr int kBeamReorderCtas = 5;  // an SM holds: 617 MB of a cache in 97 us; a sixth would wait its turn (126 us)
+constexpr int kBeamReorderCtas = 5;  // an SM holds: 597 MB of a cache in 98 us; a sixth would wait its turn (126 us)
 
 __global__ void beam_reorder_kernel(const BeamReorderArgs a, const __grid_constant__ BeamStates states);
 

@@ -9,8 +9,8 @@
 // NaN or infinity has that scale and q = 0, so what is computed from it is NaN.
 //
 // A block takes a row, reads it twice (the second time from L1 or L2) and writes it once.  512
-// rows of 4096 bf16 take 3.8 us with 16-byte loads and 5.3 us where their alignment rules
-// those out, 16 rows 2.4 and 4.4 us: latency at any size that a draft step has.
+// rows of 4096 bf16 take 3.9 us with 16-byte loads and 5.5 us where their alignment rules
+// those out, 16 rows 2.6 and 4.8 us: latency at any size that a draft step has.
 #include "i8_gemm.cuh"
 
 namespace dels {
